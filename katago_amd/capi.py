@@ -147,6 +147,51 @@ TUNING_SIGNATURES = {
     "kmx_bench_mfma_sustained": (ctypes.c_int, [ctypes.c_int] * 4 + [ctypes.c_double] + [ctypes.POINTER(ctypes.c_double)] * 2),
 }
 
+
+class RmsNormArgs(ctypes.Structure):  # include/katamx_ops.h
+    _fields_ = ([("type", ctypes.c_int32), ("scale_kind", ctypes.c_int32), ("rows", ctypes.c_int64), ("channels", ctypes.c_int32),
+                 ("epsilon", ctypes.c_float)] +
+                [(n, ctypes.c_void_p) for n in ("x", "residual", "sum", "weight", "beta", "mask", "y", "codes", "scales")] +
+                [(n, ctypes.c_int64) for n in ("x_stride", "residual_stride", "sum_stride", "y_stride", "codes_stride")])
+
+
+class Linear8Args(ctypes.Structure):
+    _fields_ = ([("out_type", ctypes.c_int32), ("scale_kind", ctypes.c_int32), ("rows", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32)] +
+                [(n, ctypes.c_void_p) for n in ("a", "a_scales", "w", "w_scales", "bias", "out")] +
+                [(n, ctypes.c_int64) for n in ("a_stride", "w_stride", "out_stride")])
+
+
+class RotaryTensor(ctypes.Structure):
+    _fields_ = ([("in_", ctypes.c_void_p), ("out", ctypes.c_void_p)] +
+                [("%s_%s_stride" % (io, d), ctypes.c_int64) for io in ("in", "out") for d in ("batch", "seq", "head")])
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = ([("type", ctypes.c_int32), ("half", ctypes.c_int32), ("inverse", ctypes.c_int32), ("magnitude", ctypes.c_float),
+                 ("batch", ctypes.c_int64), ("seq", ctypes.c_int64)] +
+                [(n, ctypes.c_int32) for n in ("q_heads", "k_heads", "head_dim", "pairs", "axes", "freq_heads")] +
+                [("frequencies", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("positions_are_64bit", ctypes.c_int32)] +
+                [("pos_%s_stride" % d, ctypes.c_int64) for d in ("batch", "seq", "axis")] + [("q", RotaryTensor), ("k", RotaryTensor)])
+
+
+# every symbol include/katamx_ops.h declares
+OPS_SIGNATURES = {
+    "kmx_ops_version": (ctypes.c_int, []),
+    "kmx_rmsnorm": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
+    "kmx_quantize": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                    ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "kmx_linear8": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
+    "kmx_rotary": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
+}
+
+
+def bind_ops(lib):
+    """Types of the operators' entry points. Apart from SIGNATURES: a library built before them (KMX_LIBRARY) still evaluates nets."""
+    for name, (res, args) in OPS_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
+
+
 _lib = None
 
 

@@ -1,0 +1,342 @@
+// norm_quant.hip — RMS norm of rows with the residual's addition in front and e4m3 with scales behind (TransformerRMSNormLayer::apply,
+// eigenbackend.cpp:885-915, between two sublayers of a transformer trunk whose projections read 8 bits), and the 8-bit form alone.
+//
+//   h_c = T(x_c + r_c)        rounded to the stream's type, because the stream is what the next sublayer adds to: the norm is of what is stored
+//   y_c = h_c * (sum_c h_c^2 / C + eps)^(-1/2) * w_c + beta_c;  0 on rows whose mask is 0
+//   SCALES_ROW  s = max(max_c |y_c| / 448, 2^-126), 1 where y is all 0;                  code_c = e4m3(y_c / s)
+//   SCALES_MX   s = 2^k with the smallest k >= -127 for which max |y| / s <= 448 over 32 channels, 1 where they are all 0
+//   A row (a block of 32) that holds an infinity or a NaN gets the scale NaN and codes 0.
+// Everything between the loads and the stores is fp32. e4m3 rounds to nearest even: 448 is its largest value, nothing clips.
+#include "device_common.h"
+#include "ops.h"
+
+namespace kmx {
+
+namespace {
+
+// Vectors at element alignment: rows of any length start anywhere. gfx950 serves unaligned 16-byte accesses; aligned ones cost the same as with
+// an aligned type.
+typedef _Float16 h16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 b16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef float f32x8u __attribute__((ext_vector_type(8), aligned(4)));
+typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(1)));
+template <class T> struct Unaligned8;
+template <> struct Unaligned8<_Float16> { typedef h16x8u V; };
+template <> struct Unaligned8<__bf16> { typedef b16x8u V; };
+template <> struct Unaligned8<float> { typedef f32x8u V; };
+
+__device__ __forceinline__ unsigned bitsOf(float x) { return __builtin_bit_cast(unsigned, x); }
+__device__ __forceinline__ float floatOf(unsigned x) { return __builtin_bit_cast(float, x); }
+
+// 8 elements from c on as fp32; those at or beyond C are 0
+template <class TR>
+__device__ __forceinline__ void load8(const typename TR::T* p, int c, int C, float (&v)[8]) {
+  if(c + 8 <= C) {
+    const typename Unaligned8<typename TR::T>::V t = *(const typename Unaligned8<typename TR::T>::V*)(p + c);
+#pragma unroll
+    for(int i = 0; i < 8; i++) v[i] = TR::toFloat(t[i]);
+  }
+  else {
+#pragma unroll
+    for(int i = 0; i < 8; i++) v[i] = c + i < C ? TR::toFloat(p[c + i]) : 0.0f;
+  }
+}
+template <class TR>
+__device__ __forceinline__ void store8(typename TR::T* p, int c, int C, const float (&v)[8]) {
+  if(c + 8 <= C) {
+    typename Unaligned8<typename TR::T>::V t;
+#pragma unroll
+    for(int i = 0; i < 8; i++) t[i] = TR::fromFloat(v[i]);
+    *(typename Unaligned8<typename TR::T>::V*)(p + c) = t;
+  }
+  else {
+#pragma unroll
+    for(int i = 0; i < 8; i++)
+      if(c + i < C) p[c + i] = TR::fromFloat(v[i]);
+  }
+}
+__device__ __forceinline__ void storeCodes8(uint8_t* p, int c, int C, const float (&v)[8], float inv) {
+  float u[8];
+#pragma unroll
+  for(int i = 0; i < 8; i++) u[i] = __builtin_fminf(__builtin_fmaxf(v[i] * inv, -E4M3_MAX), E4M3_MAX);
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(u[4], u[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(u[6], u[7], hi, true);
+  if(c + 8 <= C) {
+    u32x2u t;
+    t[0] = (unsigned)lo;
+    t[1] = (unsigned)hi;
+    *(u32x2u*)(p + c) = t;
+  }
+  else {
+#pragma unroll
+    for(int i = 0; i < 8; i++)
+      if(c + i < C) p[c + i] = (uint8_t)((unsigned)(i < 4 ? lo : hi) >> (8 * (i & 3)));
+  }
+}
+
+// |v| as bits: as unsigned numbers they are ordered as the values are, infinities and NaNs above all finite ones
+__device__ __forceinline__ unsigned maxBits(const float (&v)[8]) {
+  unsigned m = 0;
+#pragma unroll
+  for(int i = 0; i < 8; i++) {
+    const unsigned b = bitsOf(v[i]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  return m;
+}
+__device__ __forceinline__ unsigned shflXorBits(unsigned v, int mask) { return bitsOf(__shfl_xor(floatOf(v), mask)); }
+
+// The row's scale and what its values are multiplied with, from the bits of its largest magnitude
+__device__ __forceinline__ void rowScale(unsigned top, float& scale, float& inv) {
+  if(top >= 0x7f800000u) {
+    scale = floatOf(0x7fc00000u);
+    inv = 0.0f;
+  }
+  else if(top == 0) scale = inv = 1.0f;
+  else {
+    scale = floatOf(top) / E4M3_MAX;
+    if(scale < 1.17549435e-38f) scale = 1.17549435e-38f;
+    inv = 1.0f / scale;
+  }
+}
+// ... and a block's e8m0 code: top = (1 + m) 2^(e - 127), 448 = 1.75 * 2^8, so k = e - 127 - 8, one more where 1 + m > 1.75
+__device__ __forceinline__ void mxScale(unsigned top, unsigned& code, float& inv) {
+  if(top >= 0x7f800000u) {
+    code = 255;
+    inv = 0.0f;
+  }
+  else if(top == 0) {
+    code = 127;
+    inv = 1.0f;
+  }
+  else {
+    const int k = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);  // + 127
+    code = k < 0 ? 0 : (unsigned)k;
+    inv = floatOf((254u - code) << 23);  // 2^(127 - code); code <= 247
+  }
+}
+// v with the infinities and NaNs of a spoilt row replaced, so that 0 * v is 0
+__device__ __forceinline__ void zeroIf(bool spoilt, float (&v)[8]) {
+  if(!spoilt) return;
+#pragma unroll
+  for(int i = 0; i < 8; i++) v[i] = 0.0f;
+}
+
+// Sum / largest over the TPR threads of a row; up to a wave through lane exchanges, beyond it through LDS. The order is fixed: the same
+// inputs give the same bits.
+template <int TPR>
+__device__ __forceinline__ float rowSum(float v, float* part) {
+#pragma unroll
+  for(int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += __shfl_xor(v, o);
+  if constexpr(TPR > 64) {
+    if((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for(int w = 0; w < TPR / 64; w++) v += part[w];
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ unsigned rowMax(unsigned v, unsigned* part) {
+#pragma unroll
+  for(int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) {
+    const unsigned u = shflXorBits(v, o);
+    v = u > v ? u : v;
+  }
+  if constexpr(TPR > 64) {
+    if((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for(int w = 0; w < TPR / 64; w++) v = part[w] > v ? part[w] : v;
+  }
+  return v;
+}
+
+// The norm's factor applied to 8 values: v * r * w + beta, 0 on a masked row
+__device__ __forceinline__ void scale8(const NormQuantArgs& a, int c, float r, bool on, float (&v)[8]) {
+  if(!a.normed) return;
+  float w[8];
+  if(a.weight != nullptr) load8<TraitsF32>(a.weight, c, a.C, w);
+#pragma unroll
+  for(int i = 0; i < 8; i++) v[i] = v[i] * r * (a.weight != nullptr ? w[i] : 1.0f);
+  if(a.beta != nullptr) {
+    load8<TraitsF32>(a.beta, c, a.C, w);
+#pragma unroll
+    for(int i = 0; i < 8; i++) v[i] += w[i];
+  }
+  zeroIf(!on, v);
+}
+// x + residual of 8 channels, rounded to the stream's type and stored
+template <class TR>
+__device__ __forceinline__ void stream8(const NormQuantArgs& a, int64_t row, int c, float (&v)[8]) {
+  typedef typename TR::T T;
+  load8<TR>((const T*)a.x + row * a.xStride, c, a.C, v);
+  if(a.residual == nullptr) return;
+  float r[8];
+  load8<TR>((const T*)a.residual + row * a.residualStride, c, a.C, r);
+#pragma unroll
+  for(int i = 0; i < 8; i++) v[i] = TR::toFloat(TR::fromFloat(v[i] + r[i]));
+  store8<TR>((T*)a.sum + row * a.sumStride, c, a.C, v);
+}
+// 8-bit output of 8 channels whose block of 32 lies in four neighbouring lanes
+__device__ __forceinline__ void mx8(const NormQuantArgs& a, int64_t row, int c, bool in, float (&v)[8]) {
+  unsigned top = maxBits(v), u = shflXorBits(top, 1);
+  top = u > top ? u : top;
+  u = shflXorBits(top, 2);
+  top = u > top ? u : top;
+  unsigned code;
+  float inv;
+  mxScale(top, code, inv);
+  zeroIf(code == 255, v);
+  if(!in) return;
+  storeCodes8(a.codes + row * a.codesStride, c, a.C, v, inv);
+  if((c & (MX_BLOCK - 1)) == 0) ((uint8_t*)a.scales)[row * (a.C / MX_BLOCK) + c / MX_BLOCK] = (uint8_t)code;
+}
+
+// A row on TPR threads, its values in registers: 8 consecutive channels a thread and round, NCH rounds. x and residual are read once, everything
+// else is written once.
+template <class TR, int TPR, int NCH>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void normQuantKernel(NormQuantArgs a) {
+  constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+  __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const bool valid = row < a.rows;  // (lanes without a row stay for the exchanges)
+  float v[NCH][8];
+  float ss = 0.0f;
+#pragma unroll
+  for(int i = 0; i < NCH; i++) {
+    const int c = (t + i * TPR) * 8;
+    if(valid && c < a.C) stream8<TR>(a, row, c, v[i]);
+    else zeroIf(true, v[i]);
+#pragma unroll
+    for(int j = 0; j < 8; j++) ss += v[i][j] * v[i][j];
+  }
+  float r = 1.0f;
+  if(a.normed) r = rsqrtf(rowSum<TPR>(ss, part[0]) / (float)a.C + a.eps);
+  const bool on = a.mask == nullptr || !valid || a.mask[row] != 0.0f;
+  unsigned top = 0;
+#pragma unroll
+  for(int i = 0; i < NCH; i++) {
+    const int c = (t + i * TPR) * 8;
+    if(valid && c < a.C) {
+      scale8(a, c, r, on, v[i]);
+      if(a.y != nullptr) store8<TR>((typename TR::T*)a.y + row * a.yStride, c, a.C, v[i]);
+    }
+    if(a.scaleKind == SCALES_ROW) {
+      const unsigned m = maxBits(v[i]);
+      top = m > top ? m : top;
+    }
+  }
+  if(a.scaleKind == SCALES_ROW) {
+    top = rowMax<TPR>(top, (unsigned*)part[1]);
+    float scale, inv;
+    rowScale(top, scale, inv);
+#pragma unroll
+    for(int i = 0; i < NCH; i++) {
+      const int c = (t + i * TPR) * 8;
+      if(!valid || c >= a.C) continue;
+      zeroIf(inv == 0.0f, v[i]);
+      storeCodes8(a.codes + row * a.codesStride, c, a.C, v[i], inv);
+    }
+    if(valid && t == 0) ((float*)a.scales)[row] = scale;
+  }
+  else if(a.scaleKind == SCALES_MX) {
+#pragma unroll
+    for(int i = 0; i < NCH; i++) {
+      const int c = (t + i * TPR) * 8;
+      mx8(a, row, c, valid && c < a.C, v[i]);
+    }
+  }
+}
+
+// Rows longer than the registers hold: a work-group of 1024 walks the row up to three times (sum of squares, largest magnitude, outputs); after the
+// first walk it reads what it wrote itself. Rows are long enough here that later walks mostly hit the caches.
+template <class TR>
+__global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
+  typedef typename TR::T T;
+  constexpr int TPR = 1024;
+  __shared__ float part[2][TPR / 64];
+  const int64_t row = blockIdx.x;
+  const T* const h = a.residual != nullptr ? (const T*)a.sum + row * a.sumStride : (const T*)a.x + row * a.xStride;
+  float v[8];
+  float r = 1.0f;
+  if(a.normed) {
+    float ss = 0.0f;
+    for(int c = threadIdx.x * 8; c < a.C; c += TPR * 8) {
+      stream8<TR>(a, row, c, v);
+#pragma unroll
+      for(int j = 0; j < 8; j++) ss += v[j] * v[j];
+    }
+    r = rsqrtf(rowSum<TPR>(ss, part[0]) / (float)a.C + a.eps);
+  }
+  const bool on = a.mask == nullptr || a.mask[row] != 0.0f;
+  float scale = 1.0f, inv = 1.0f;
+  if(a.scaleKind == SCALES_ROW) {
+    unsigned top = 0;
+    for(int c = threadIdx.x * 8; c < a.C; c += TPR * 8) {
+      load8<TR>(h, c, a.C, v);
+      scale8(a, c, r, on, v);
+      const unsigned m = maxBits(v);
+      top = m > top ? m : top;
+    }
+    rowScale(rowMax<TPR>(top, (unsigned*)part[1]), scale, inv);
+    if(threadIdx.x == 0) ((float*)a.scales)[row] = scale;
+  }
+  for(int c0 = 0; c0 < a.C; c0 += TPR * 8) {  // (all lanes take part in a block's exchanges)
+    const int c = c0 + threadIdx.x * 8;
+    const bool in = c < a.C;
+    zeroIf(true, v);
+    if(in) {
+      load8<TR>(h, c, a.C, v);
+      scale8(a, c, r, on, v);
+      if(a.y != nullptr) store8<TR>((T*)a.y + row * a.yStride, c, a.C, v);
+    }
+    if(a.scaleKind == SCALES_ROW && in) {
+      zeroIf(inv == 0.0f, v);
+      storeCodes8(a.codes + row * a.codesStride, c, a.C, v, inv);
+    }
+    else if(a.scaleKind == SCALES_MX) mx8(a, row, c, in, v);
+  }
+}
+
+template <class TR, int TPR, int NCH>
+void launchRows(const NormQuantArgs& a, hipStream_t stream) {
+  constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+  auto kern = normQuantKernel<TR, TPR, NCH>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, stream, a);
+}
+template <class TR>
+void launchOne(const NormQuantArgs& a, hipStream_t stream) {
+  const int pieces = (a.C + 7) / 8;
+  if(pieces <= 16) launchRows<TR, 16, 1>(a, stream);
+  else if(pieces <= 32) launchRows<TR, 16, 2>(a, stream);
+  else if(pieces <= 64) launchRows<TR, 16, 4>(a, stream);
+  else if(pieces <= 128) launchRows<TR, 64, 2>(a, stream);
+  else if(pieces <= 256) launchRows<TR, 64, 4>(a, stream);
+  else if(pieces <= 512) launchRows<TR, 256, 2>(a, stream);
+  else if(pieces <= 1024) launchRows<TR, 256, 4>(a, stream);
+  else if(pieces <= 4096) launchRows<TR, 1024, 4>(a, stream);
+  else {
+    auto kern = normQuantLongKernel<TR>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+  }
+}
+
+}  // namespace
+
+hipError_t launchNormQuant(int dtype, const NormQuantArgs& a, hipStream_t stream) {
+  if(a.rows == 0) return hipSuccess;
+  if(dtype == DT_F16) launchOne<TraitsF16>(a, stream);
+  else if(dtype == DT_BF16) launchOne<TraitsBF16>(a, stream);
+  else if(dtype == DT_F32) launchOne<TraitsF32>(a, stream);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+}  // namespace kmx
