@@ -26,21 +26,37 @@ typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 constexpr int KSTEP = 128;  // k of one step: a row of 128 bytes in LDS, eight pieces of 16
 constexpr int KPIECES = 8;
 
-__device__ __attribute__((aligned(16))) unsigned linear8Zeros[4];  // what pieces beyond K are fetched from
-
 #ifdef KMX_EMULATED_HIP
 inline unsigned ldsAddress(void* p) { return (unsigned)(size_t)p; }
-inline void dma16(const void* src, unsigned dst) { emu::globalLoadLds((size_t)src, (size_t)dst, 16, 0, 0); }
+typedef const char* Rsrc;
+inline Rsrc bufferOf(const void* p) { return (const char*)p; }
+inline void dma16(Rsrc b, unsigned off, unsigned step, unsigned dst) { emu::globalLoadLds((size_t)b + off + step, (size_t)dst, 16, 0, 0); }
 inline u32x4 ldsRead16(unsigned at) { return *(const u32x4*)(size_t)at; }
 inline void waitLoads0() { emu::waitVm(0); }
+inline void waitReads0() {}
+inline void waveBarrier() { __syncthreads(); }
 #else
 __device__ __forceinline__ unsigned ldsAddress(void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) char*)p; }
-__device__ __forceinline__ void dma16(const void* src, unsigned dst) {  // lane l's 16 bytes land at dst + 16 l; dst is uniform
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)(size_t)dst, 16, 0, 0);
+// LDS-DMA: the 16 bytes at off (a lane's own) + step (uniform) of a buffer land at dst (uniform) + 16 lane. (As a buffer and not by pointers: no 64-bit
+// address for each request and lane, which took more registers than there are.)
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ Rsrc bufferOf(const void* p) {  // p is uniform; said again, because a request on a descriptor in vector registers is a loop over lanes
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)(size_t)p), hi = __builtin_amdgcn_readfirstlane((unsigned)((size_t)p >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((size_t)hi << 32 | lo), 0, 0xffffffff, 0x00027000);
+}
+__device__ __forceinline__ void dma16(Rsrc b, unsigned off, unsigned step, unsigned dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)(size_t)dst, 16, off, step, 0, 0);
 }
 __device__ __forceinline__ u32x4 ldsRead16(unsigned at) { return *(const __attribute__((address_space(3))) u32x4*)(size_t)at; }
 __device__ __forceinline__ void waitLoads0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void waitReads0() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void waveBarrier() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 #endif
+
+template <int I> struct Index { static constexpr int value = I; };
 
 template <int OUT> struct OutTraits;
 template <> struct OutTraits<DT_F16> { typedef TraitsF16 TR; };
@@ -59,10 +75,28 @@ __device__ __forceinline__ float ofE8m0(unsigned code) {  // 2^(code - 127); 0 i
   return __builtin_bit_cast(float, code == 0 ? 0x00400000u : code == 255 ? 0x7fc00000u : code << 23);
 }
 
+typedef unsigned u32u __attribute__((aligned(1)));
+// A row's e8m0 codes of one step, a byte for each 32 k; beyond the row's end 0 (their weights are zeros). The word is fetched in one piece - so that
+// the main loop stays one block, in whose order the products and the barrier stay where they are written - and shifted when it is used.
+__device__ __forceinline__ int codesAt(int blocks, int step) { return step * 4 < blocks - 4 ? step * 4 : blocks - 4; }
+__device__ __forceinline__ unsigned fetchCodes(const uint8_t* p, int blocks, int step) { return *(const u32u*)(p + codesAt(blocks, step)); }
+__device__ __forceinline__ unsigned shiftedCodes(unsigned word, int blocks, int step) { return word >> (8 * (step * 4 - codesAt(blocks, step))); }
+
+// 4 floats from p[c] on, those beyond `last` as p[last]
+__device__ __forceinline__ f32x4 fourFloats(const float* p, int c, int last) {
+  if(c + 3 <= last) return *(const f32x4u*)(p + c);
+  f32x4 v;
+#pragma unroll
+  for(int i = 0; i < 4; i++) v[i] = p[c + i < last ? c + i : last];
+  return v;
+}
+
 // One BM x BN tile of the output on WM x WN waves. Steps of 128 k: the rows of a and w lie in LDS as they lie in memory, 128 bytes each, the eight
 // pieces of row r at piece ^ ((r >> 1) & 7): the 16 lanes that a ds_read_b128 serves at a time then touch all 64 banks. The pieces are brought
-// by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages, the next step's requests behind the barrier that opens
-// this step. The weights are the matrix instruction's A operand: a lane ends with consecutive output channels of one row of a and stores 16 bytes.
+// by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages. A step multiplies two halves of 64 k: a row tile's fragments
+// are replaced by the next half's as soon as they are used up, the weights' have two sets; the barrier stands behind the second half's first
+// products, when the stage has been read out - it is requested anew there, a whole step ahead of its use. The weights are the matrix instruction's A
+// operand: a lane ends with consecutive output channels of one row of a and stores 16 bytes.
 template <int BM, int BN, int WM, int WN, bool MX, int OUT>
 __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   typedef typename OutTraits<OUT>::TR TR;
@@ -70,66 +104,67 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   constexpr bool EXACT = OUT == DT_F32;
   constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
   constexpr int REQ_A = BM / 8 / NW, REQ_W = BN / 8 / NW;  // requests of a wave and step, 8 rows each
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && TM % 32 == 0 && TN % 32 == 0, "tile");
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && TM % 32 == 0 && TN % 32 == 0 && BM + BN <= 64 * NW, "tile");
   constexpr unsigned STAGE = (unsigned)(BM + BN) * KSTEP;
   HIP_DYNAMIC_SHARED(f32x4, smemLinear8)
   const unsigned lds = ldsAddress(smemLinear8);
+  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + 2 * STAGE);  // [2][BM + BN]: a step's e8m0 codes of each row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hh = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
-  const unsigned nTiles = (unsigned)(g.N + BN - 1) / BN;
-  const int64_t m0 = (int64_t)(blockIdx.x / nTiles) * BM;
-  const int n0 = (int)(blockIdx.x % nTiles) * BN;
+
+  // Work-groups go round the 8 XCDs one by one: each XCD takes a contiguous eighth of the tiles, in strips of 8 tiles of rows, so that what runs at
+  // a time on an XCD shares rows of a and of w in its L2
+  const unsigned mTiles = (unsigned)((g.rows + BM - 1) / BM), nTiles = (unsigned)(g.N + BN - 1) / BN;
+  unsigned tile = blockIdx.x;
+  {
+    const unsigned all = mTiles * nTiles, xcd = tile & 7, each = all >> 3, more = all & 7;
+    tile = xcd * each + (xcd < more ? xcd : more) + (tile >> 3);
+  }
+  const unsigned strip = tile / (8 * nTiles), in = tile % (8 * nTiles), tall = mTiles - strip * 8 < 8 ? mTiles - strip * 8 : 8;
+  const int64_t m0 = (int64_t)(strip * 8 + in % tall) * BM;
+  const int n0 = (int)(in / tall) * BN;
   const int steps = (g.K + KSTEP - 1) / KSTEP, pieces = g.K / 16;
   const int mLast = (int)(g.rows - m0 < BM ? g.rows - m0 : BM) - 1, nLast = (g.N - n0 < BN ? g.N - n0 : BN) - 1;  // of this tile
 
   // rows beyond the matrix are fetched from its last row: their products end in rows / channels that are not stored
   const uint8_t* const aTile = g.a + m0 * g.aStride;
   const uint8_t* const wTile = g.w + (int64_t)n0 * g.wStride;
-  unsigned off[REQ_A + REQ_W], piece[REQ_A + REQ_W];
+  unsigned off[REQ_A + REQ_W];
+  auto pieceOf = [&](int r) { return (lane & 7) ^ ((r >> 1) & 7); };
+  auto rowOf = [&](int j) { return (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8 + (lane >> 3); };
 #pragma unroll
   for(int j = 0; j < REQ_A + REQ_W; j++) {
-    const int r = (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8 + (lane >> 3), last = j < REQ_A ? mLast : nLast;
-    piece[j] = (unsigned)((lane & 7) ^ ((r >> 1) & 7));
-    off[j] = (unsigned)(r < last ? r : last) * (unsigned)(j < REQ_A ? g.aStride : g.wStride) + piece[j] * 16;
+    const int r = rowOf(j), last = j < REQ_A ? mLast : nLast;
+    off[j] = (unsigned)(r < last ? r : last) * (unsigned)(j < REQ_A ? g.aStride : g.wStride) + (unsigned)pieceOf(r) * 16;
   }
-  auto issue = [&](int step) {
+  const Rsrc aRsrc = bufferOf(aTile), wRsrc = bufferOf(wTile);
+  // CUT: the step that holds the end of K. Pieces beyond it are fetched as the row's last one; the weights' are zeroed before they are multiplied
+  auto issue = [&](int step, auto cutTag) {
     const unsigned stage = lds + (unsigned)(step & 1) * STAGE;
-    const bool whole = (step + 1) * KPIECES <= pieces;
 #pragma unroll
     for(int j = 0; j < REQ_A + REQ_W; j++) {
-      const uint8_t* src = (j < REQ_A ? aTile : wTile) + (size_t)step * KSTEP + off[j];
-      if(!whole && step * KPIECES + (int)piece[j] >= pieces) src = (const uint8_t*)linear8Zeros;
-      dma16(src, stage + (unsigned)((j < REQ_A ? 0 : BM) + (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8) * KSTEP);
+      const unsigned dst = stage + (unsigned)((j < REQ_A ? 0 : BM) + (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8) * KSTEP;
+      unsigned from = off[j];
+      if constexpr(decltype(cutTag)::value != 0) {
+        const int over = step * KPIECES + pieceOf(rowOf(j)) - (pieces - 1);
+        from -= over > 0 ? (unsigned)over * 16 : 0;
+      }
+      dma16(j < REQ_A ? aRsrc : wRsrc, from, (unsigned)step * KSTEP, dst);
     }
   };
 
-  // a step's four e8m0 codes of this lane's rows, one byte for each 32 k
+  // e8m0 codes: a thread fetches one row's of a step and puts them into LDS half a step later
   const int blocks = MX ? g.K / MX_BLOCK : 0;
-  unsigned aCodes[MX ? MI : 1], wCodes[MX ? NI : 1];
-  auto fourCodes = [&](const void* scales, int64_t row, int step) {
-    const uint8_t* const p = (const uint8_t*)scales + row * blocks;
-    unsigned v = 0;
-#pragma unroll
-    for(int q = 0; q < 4; q++) {
-      const int blk = step * 4 + q;
-      v |= (blk < blocks ? (unsigned)p[blk] : 127u) << (8 * q);
-    }
-    return v;
-  };
-  auto loadCodes = [&](int step) {
-    if constexpr(MX) {
-#pragma unroll
-      for(int mi = 0; mi < MI; mi++) {
-        const int r = wm * TM + mi * 32 + col;
-        aCodes[mi] = fourCodes(g.aScales, m0 + (r < mLast ? r : mLast), step);
-      }
-#pragma unroll
-      for(int ni = 0; ni < NI; ni++) {
-        const int r = wn * TN + ni * 32 + col;
-        wCodes[ni] = fourCodes(g.wScales, n0 + (r < nLast ? r : nLast), step);
-      }
-    }
+  const int codeRow = (int)threadIdx.x < BM + BN ? (int)threadIdx.x : BM + BN - 1;
+  const uint8_t* myCodes = nullptr;
+  if constexpr(MX) {
+    if(codeRow < BM) myCodes = (const uint8_t*)g.aScales + (m0 + (codeRow < mLast ? codeRow : mLast)) * blocks;
+    else myCodes = (const uint8_t*)g.wScales + (int64_t)(n0 + (codeRow - BM < nLast ? codeRow - BM : nLast)) * blocks;
+  }
+  unsigned fetched = 0;
+  auto putCodes = [&](int step) {
+    if constexpr(MX) codesOf[(step & 1) * (BM + BN) + codeRow] = shiftedCodes(fetched, blocks, step);
   };
 
   f32x16 acc[NI][MI];
@@ -141,99 +176,185 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
       for(int v = 0; v < 16; v++) acc[ni][mi][v] = 0.0f;
 
   const unsigned swz = (unsigned)(col >> 1) & 7u;
-  issue(0);
-  for(int step = 0; step < steps; step++) {
-    loadCodes(step);
-    waitLoads0();
-    __builtin_amdgcn_s_barrier();  // this step's pieces are there, and nobody reads the other stage any more
-    if(step + 1 < steps) issue(step + 1);
-    const unsigned stage = lds + (unsigned)(step & 1) * STAGE;
-    const unsigned aRows = stage + (unsigned)(wm * TM + col) * KSTEP, wRows = stage + (unsigned)(BM + wn * TN + col) * KSTEP;
+  // a step is two halves of 64 k; s = 0, 1: pieces 4 s + hh (k 0..31 of the half) and 4 s + 2 + hh (k 32..63)
+  u32x4 fa[MI][2], fw[2][NI][2];
+  auto rowsOf = [&](int step, int base) { return lds + (unsigned)(step & 1) * STAGE + (unsigned)(base + col) * KSTEP; };
+  auto pieceAt = [&](int p) { return ((unsigned)(p + hh) ^ swz) * 16; };
+  auto readA = [&](int step, int s, int mi) {
+    const unsigned rows = rowsOf(step, wm * TM) + mi * 32 * KSTEP;
+    fa[mi][0] = ldsRead16(rows + pieceAt(4 * s));
+    fa[mi][1] = ldsRead16(rows + pieceAt(4 * s + 2));
+  };
+  auto readW = [&](int step, int s) {
+    const unsigned rows = rowsOf(step, BM + wn * TN);
 #pragma unroll
-    for(int s = 0; s < 2; s++) {  // 64 k: pieces 4 s + hh (k 0..31 of them) and 4 s + 2 + hh (k 32..63)
-      const unsigned c0 = ((unsigned)(4 * s + hh) ^ swz) * 16, c1 = ((unsigned)(4 * s + 2 + hh) ^ swz) * 16;
-      u32x4 fa[MI][2], fw[NI][2];
+    for(int ni = 0; ni < NI; ni++) {
+      fw[s][ni][0] = ldsRead16(rows + ni * 32 * KSTEP + pieceAt(4 * s));
+      fw[s][ni][1] = ldsRead16(rows + ni * 32 * KSTEP + pieceAt(4 * s + 2));
+    }
+  };
+  // The instruction takes the scale of k 0..31 from lanes 0..31 and that of k 32..63 from lanes 32..63: its byte 2 s of a step's four, shifted by hh
+  // here. (The bf16 way needs both of a half's in every lane.)
+  unsigned aCodes[MX ? MI : 1], wCodes[MX ? NI : 1], aNext[MX ? MI : 1], wNext[MX ? NI : 1];
+  auto readCodes = [&](int step) {
+    if constexpr(MX) {
+      const unsigned* const c = codesOf + (step & 1) * (BM + BN);
 #pragma unroll
-      for(int mi = 0; mi < MI; mi++) {
-        fa[mi][0] = ldsRead16(aRows + mi * 32 * KSTEP + c0);
-        fa[mi][1] = ldsRead16(aRows + mi * 32 * KSTEP + c1);
-      }
+      for(int mi = 0; mi < MI; mi++) aNext[mi] = c[wm * TM + mi * 32 + col] >> (EXACT ? 0 : 8 * hh);
 #pragma unroll
-      for(int ni = 0; ni < NI; ni++) {
-        fw[ni][0] = ldsRead16(wRows + ni * 32 * KSTEP + c0);
-        fw[ni][1] = ldsRead16(wRows + ni * 32 * KSTEP + c1);
-      }
-      if constexpr(EXACT) {
+      for(int ni = 0; ni < NI; ni++) wNext[ni] = c[BM + wn * TN + ni * 32 + col] >> (EXACT ? 0 : 8 * hh);
+    }
+  };
+  auto takeCodes = [&]() {
+    if constexpr(MX) {
 #pragma unroll
-        for(int q = 0; q < 4; q++) {  // 16 k: 8 codes of each half wave
-          const int blk = 2 * s + (q >> 1);
-          Bf8 ba[MI], bw[NI];
+      for(int mi = 0; mi < MI; mi++) aCodes[mi] = aNext[mi];
 #pragma unroll
-          for(int mi = 0; mi < MI; mi++)
-            ba[mi] = bf16Of(fa[mi][q >> 1][2 * (q & 1)], fa[mi][q >> 1][2 * (q & 1) + 1], MX ? ofE8m0(aCodes[mi] >> (8 * blk) & 255u) : 1.0f);
+      for(int ni = 0; ni < NI; ni++) wCodes[ni] = wNext[ni];
+    }
+  };
+  auto multiply = [&](auto sTag, int mi) {
+    constexpr int s = decltype(sTag)::value;
+    if constexpr(EXACT) {
 #pragma unroll
-          for(int ni = 0; ni < NI; ni++)
-            bw[ni] = bf16Of(fw[ni][q >> 1][2 * (q & 1)], fw[ni][q >> 1][2 * (q & 1) + 1], MX ? ofE8m0(wCodes[ni] >> (8 * blk) & 255u) : 1.0f);
-#pragma unroll
-          for(int ni = 0; ni < NI; ni++)
-#pragma unroll
-            for(int mi = 0; mi < MI; mi++) acc[ni][mi] = TraitsBF16::mfma(bw[ni], ba[mi], acc[ni][mi]);
-        }
-      }
-      else {
-        // the instruction takes the scale of k 0..31 from lanes 0..31 and that of k 32..63 from lanes 32..63: byte hh of the pair of blocks
-        constexpr int UNIT = 0x7f7f7f7f;
-        i32x8 xa[MI], xw[NI];
-#pragma unroll
-        for(int mi = 0; mi < MI; mi++)
-#pragma unroll
-          for(int i = 0; i < 8; i++) xa[mi][i] = (int)fa[mi][i >> 2][i & 3];
+      for(int q = 0; q < 4; q++) {  // 16 k: 8 codes of each half wave
+        const int blk = 2 * s + (q >> 1), e = 2 * (q & 1);
+        const Bf8 ba = bf16Of(fa[mi][q >> 1][e], fa[mi][q >> 1][e + 1], MX ? ofE8m0(aCodes[MX ? mi : 0] >> (8 * blk) & 255u) : 1.0f);
 #pragma unroll
         for(int ni = 0; ni < NI; ni++)
-#pragma unroll
-          for(int i = 0; i < 8; i++) xw[ni][i] = (int)fw[ni][i >> 2][i & 3];
-#pragma unroll
-        for(int ni = 0; ni < NI; ni++)
-#pragma unroll
-          for(int mi = 0; mi < MI; mi++)
-            acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw[ni], xa[mi], acc[ni][mi], 0, 0, 0,
-                                                                          MX ? (int)(wCodes[ni] >> (16 * s + 8 * hh)) : UNIT, 0,
-                                                                          MX ? (int)(aCodes[mi] >> (16 * s + 8 * hh)) : UNIT);
+          acc[ni][mi] = TraitsBF16::mfma(bf16Of(fw[s][ni][q >> 1][e], fw[s][ni][q >> 1][e + 1], MX ? ofE8m0(wCodes[MX ? ni : 0] >> (8 * blk) & 255u) : 1.0f), ba,
+                                         acc[ni][mi]);
       }
     }
+    else {
+      constexpr int UNIT = 0x7f7f7f7f;
+      i32x8 xa;
+#pragma unroll
+      for(int i = 0; i < 8; i++) xa[i] = (int)fa[mi][i >> 2][i & 3];
+#pragma unroll
+      for(int ni = 0; ni < NI; ni++) {
+        i32x8 xw;
+#pragma unroll
+        for(int i = 0; i < 8; i++) xw[i] = (int)fw[s][ni][i >> 2][i & 3];
+        acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw, xa, acc[ni][mi], 0, 0, 2 * s, MX ? (int)wCodes[MX ? ni : 0] : UNIT, 2 * s,
+                                                                      MX ? (int)aCodes[MX ? mi : 0] : UNIT);
+      }
+    }
+  };
+
+  const int wholeSteps = pieces / KPIECES;  // steps or steps - 1
+  auto issueAny = [&](int step) {
+    if(step < wholeSteps) issue(step, Index<0>());
+    else issue(step, Index<1>());
+  };
+  auto zeroBeyond = [&](int step, int s) {  // (whatever the rows of a hold there: finite, or a NaN that the row has anyway)
+#pragma unroll
+    for(int b = 0; b < 2; b++)
+      if(step * KPIECES + 4 * s + 2 * b + hh >= pieces) {
+#pragma unroll
+        for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+          for(int i = 0; i < 4; i++) fw[s][ni][b][i] = 0;
+      }
+  };
+  constexpr int NOTHING = 0, WHOLE = 1, CUT = 2;  // what a step requests for two steps on
+  auto body = [&](int step, auto moreTag, auto requestTag) {
+    constexpr bool MORE = decltype(moreTag)::value != 0;
+    constexpr int REQUEST = decltype(requestTag)::value;
+    takeCodes();
+    readW(step, 1);
+    if constexpr(!MORE)
+      if(wholeSteps < steps) {
+        zeroBeyond(step, 0);
+        zeroBeyond(step, 1);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for(int mi = 0; mi < MI; mi++) {
+      multiply(Index<0>(), mi);
+      __builtin_amdgcn_sched_barrier(0);  // (the fragment's registers are free now)
+      readA(step, 1, mi);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr(MORE) putCodes(step + 1);
+    multiply(Index<1>(), 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr(MORE) {
+      waitLoads0();   // the next stage is there,
+      waitReads0();   // this one has been read out by this wave,
+      waveBarrier();  // by all of them
+      if constexpr(REQUEST != NOTHING) {
+        if constexpr(MX) fetched = fetchCodes(myCodes, blocks, step + 2);
+        issue(step + 2, Index<REQUEST == CUT ? 1 : 0>());
+      }
+      readCodes(step + 1);
+      readW(step + 1, 0);
+      readA(step + 1, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for(int mi = 1; mi < MI; mi++) {
+      multiply(Index<1>(), mi);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr(MORE) readA(step + 1, 0, mi);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if constexpr(MX) {
+    if(blocks >= 4) fetched = fetchCodes(myCodes, blocks, 0);
+    else
+      for(int q = 0; q < blocks; q++) fetched |= (unsigned)myCodes[q] << (8 * (q + 4 - blocks));  // (as the shifted word)
   }
+  issueAny(0);
+  putCodes(0);
+  waitLoads0();
+  waitReads0();
+  waveBarrier();
+  if(steps > 1) {
+    if constexpr(MX) fetched = fetchCodes(myCodes, blocks, 1);
+    issueAny(1);
+  }
+  readCodes(0);
+  readW(0, 0);
+#pragma unroll
+  for(int mi = 0; mi < MI; mi++) readA(0, 0, mi);
+  int step = 0;
+  for(; step + 2 < wholeSteps; step++) body(step, Index<1>(), Index<WHOLE>());
+  if(step + 2 < steps) body(step++, Index<1>(), Index<CUT>());
+  if(step + 1 < steps) body(step++, Index<1>(), Index<NOTHING>());
+  body(step, Index<0>(), Index<NOTHING>());
 
   // element v of a lane: channel 8 (v / 4) + 4 hh + v % 4 of the 32, row `col`
+  float sa[MI];
 #pragma unroll
   for(int mi = 0; mi < MI; mi++) {
     const int r = wm * TM + mi * 32 + col;
-    const bool rowIn = r <= mLast;
-    const float sa = MX ? 1.0f : ((const float*)g.aScales)[m0 + (rowIn ? r : mLast)];
-    TO* const row = (TO*)g.out + (m0 + r) * g.outStride + n0;
+    sa[mi] = MX ? 1.0f : ((const float*)g.aScales)[m0 + (r < mLast ? r : mLast)];
+  }
 #pragma unroll
-    for(int ni = 0; ni < NI; ni++) {
-      const int c0 = wn * TN + ni * 32;
+  for(int ni = 0; ni < NI; ni++) {
+    const int c0 = wn * TN + ni * 32;
+    f32x4 sw[4], bias[4];
+#pragma unroll
+    for(int q = 0; q < 4; q++) {
+      sw[q] = MX ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : fourFloats((const float*)g.wScales + n0, c0 + 8 * q + 4 * hh, nLast);
+      bias[q] = g.bias == nullptr ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : fourFloats(g.bias + n0, c0 + 8 * q + 4 * hh, nLast);
+    }
+#pragma unroll
+    for(int mi = 0; mi < MI; mi++) {
+      const int r = wm * TM + mi * 32 + col;
+      TO* const row = (TO*)g.out + (m0 + r) * g.outStride + n0;
       u32x2 pk[4];
 #pragma unroll
       for(int q = 0; q < 4; q++) {
-        const int c = c0 + 8 * q + 4 * hh;
-        float o[4];
+        f32x4 o;
 #pragma unroll
-        for(int i = 0; i < 4; i++) {
-          const int n = n0 + (c + i < nLast ? c + i : nLast);
-          float x = acc[ni][mi][4 * q + i] * sa;
-          if(!MX) x *= ((const float*)g.wScales)[n];
-          if(g.bias != nullptr) x += g.bias[n];
-          o[i] = x;
-        }
+        for(int i = 0; i < 4; i++) o[i] = acc[ni][mi][4 * q + i] * sa[mi] * sw[q][i] + bias[q][i];
         if constexpr(OUT == DT_F32) {
-          if(rowIn && c + 3 <= nLast) {
-            f32x4 t;
-#pragma unroll
-            for(int i = 0; i < 4; i++) t[i] = o[i];
-            *(f32x4u*)(row + c) = t;
-          }
-          else if(rowIn)
+          const int c = c0 + 8 * q + 4 * hh;
+          if(r <= mLast && c + 3 <= nLast) *(f32x4u*)(row + c) = o;
+          else if(r <= mLast)
             for(int i = 0; i < 4 && c + i <= nLast; i++) row[c + i] = o[i];
         }
         else {
@@ -249,8 +370,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
 #pragma unroll
         for(int j = 0; j < 2; j++) {
           const int c = c0 + 16 * j + 8 * hh;
-          if(rowIn && c + 7 <= nLast) *(u32x4u*)(row + c) = whole[j];
-          else if(rowIn) {
+          if(r <= mLast && c + 7 <= nLast) *(u32x4u*)(row + c) = whole[j];
+          else if(r <= mLast) {
             const typename TR::V8 t = __builtin_bit_cast(typename TR::V8, whole[j]);
 #pragma unroll
             for(int i = 0; i < 8; i++)
@@ -258,6 +379,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
           }
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -266,14 +388,30 @@ template <int BM, int BN, int WM, int WN, bool MX, int OUT>
 hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const int64_t tiles = (g.rows + BM - 1) / BM * ((g.N + BN - 1) / BN);
   if(tiles > 0x7fffffff) return hipErrorInvalidValue;
+  constexpr int LDS = 2 * (BM + BN) * (KSTEP + 4);
   auto kern = linear8Kernel<BM, BN, WM, WN, MX, OUT>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * WM * WN), 2 * (BM + BN) * KSTEP, stream, g);
+  if(LDS > 64 * 1024) {  // opt in to the large LDS window, once per instantiation and device
+    constexpr int MAX_DEVICES = 64;
+    static std::atomic<bool> attrSet[MAX_DEVICES];
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if(e != hipSuccess) return e;
+    if(dev < 0 || dev >= MAX_DEVICES) return hipErrorInvalidDevice;
+    if(!attrSet[dev].load(std::memory_order_acquire)) {
+      e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+      if(e != hipSuccess) return e;
+      attrSet[dev].store(true, std::memory_order_release);
+    }
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * WM * WN), LDS, stream, g);
   return hipGetLastError();
 }
 template <bool MX, int OUT>
 hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
-  const int64_t tiles128 = (g.rows + 127) / 128 * ((g.N + 127) / 128);
-  if(tiles128 >= 256) return launchTile<128, 128, 2, 2, MX, OUT>(g, stream);
+  auto tiles = [&](int bm, int bn) { return (g.rows + bm - 1) / bm * ((g.N + bn - 1) / bn); };
+  if constexpr(OUT != DT_F32)
+    if(tiles(256, 256) >= 256) return launchTile<256, 256, 2, 4, MX, OUT>(g, stream);
+  if(tiles(128, 128) >= 256) return launchTile<128, 128, 2, 2, MX, OUT>(g, stream);
   return launchTile<64, 64, 2, 2, MX, OUT>(g, stream);
 }
 template <int OUT>

@@ -83,7 +83,7 @@ inline F16 mfmaScale(I8 a, I8 b, F16 c, int sa, int sb) {
 }  // namespace emu
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) emu::cvtPkFp8(a, b, old, hi)
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, hi) emu::cvtBf16Fp8(src, scale, hi)
-#define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) emu::mfmaScale(a, b, c, sa, sb)
+#define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) emu::mfmaScale(a, b, c, (int)((unsigned)(sa) >> (8 * (oa))), (int)((unsigned)(sb) >> (8 * (ob))))
 
 #include "../../katago_amd/csrc/norm_quant.hip"
 #include "../../katago_amd/csrc/linear8.hip"
