@@ -19,8 +19,7 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef b16x8 Bf8;
-typedef u32x4 u32x4u __attribute__((aligned(2)));
-typedef f32x4 f32x4u __attribute__((aligned(4)));
+typedef u32x4 Out16 __attribute__((aligned(2)));  // 16 bytes of an output row, which starts at any element
 typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KSTEP = 128;  // k of one step: a row of 128 bytes in LDS, eight pieces of 16
@@ -31,8 +30,9 @@ inline unsigned ldsAddress(void* p) { return (unsigned)(size_t)p; }
 typedef const char* Rsrc;
 inline Rsrc bufferOf(const void* p) { return (const char*)p; }
 inline void dma16(Rsrc b, unsigned off, unsigned step, unsigned dst) { emu::globalLoadLds((size_t)b + off + step, (size_t)dst, 16, 0, 0); }
+inline void ldsWrite16(unsigned at, u32x4 v) { *(u32x4*)(size_t)at = v; }
 inline u32x4 ldsRead16(unsigned at) { return *(const u32x4*)(size_t)at; }
-inline void waitLoads0() { emu::waitVm(0); }
+template <int N> inline void waitLoads() { emu::waitVm(N); }
 inline void waitReads0() {}
 inline void waveBarrier() { __syncthreads(); }
 #else
@@ -48,7 +48,9 @@ __device__ __forceinline__ void dma16(Rsrc b, unsigned off, unsigned step, unsig
   __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)(size_t)dst, 16, off, step, 0, 0);
 }
 __device__ __forceinline__ u32x4 ldsRead16(unsigned at) { return *(const __attribute__((address_space(3))) u32x4*)(size_t)at; }
-__device__ __forceinline__ void waitLoads0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void ldsWrite16(unsigned at, u32x4 v) { *(__attribute__((address_space(3))) u32x4*)(size_t)at = v; }
+template <int N>
+__device__ __forceinline__ void waitLoads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void waitReads0() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void waveBarrier() {
   __builtin_amdgcn_s_barrier();
@@ -82,15 +84,6 @@ __device__ __forceinline__ int codesAt(int blocks, int step) { return step * 4 <
 __device__ __forceinline__ unsigned fetchCodes(const uint8_t* p, int blocks, int step) { return *(const u32u*)(p + codesAt(blocks, step)); }
 __device__ __forceinline__ unsigned shiftedCodes(unsigned word, int blocks, int step) { return word >> (8 * (step * 4 - codesAt(blocks, step))); }
 
-// 4 floats from p[c] on, those beyond `last` as p[last]
-__device__ __forceinline__ f32x4 fourFloats(const float* p, int c, int last) {
-  if(c + 3 <= last) return *(const f32x4u*)(p + c);
-  f32x4 v;
-#pragma unroll
-  for(int i = 0; i < 4; i++) v[i] = p[c + i < last ? c + i : last];
-  return v;
-}
-
 // One BM x BN tile of the output on WM x WN waves. Steps of 128 k: the rows of a and w lie in LDS as they lie in memory, 128 bytes each, the eight
 // pieces of row r at piece ^ ((r >> 1) & 7): the 16 lanes that a ds_read_b128 serves at a time then touch all 64 banks. The pieces are brought
 // by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages. A step multiplies two halves of 64 k: a row tile's fragments
@@ -108,7 +101,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   constexpr unsigned STAGE = (unsigned)(BM + BN) * KSTEP;
   HIP_DYNAMIC_SHARED(f32x4, smemLinear8)
   const unsigned lds = ldsAddress(smemLinear8);
-  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + 2 * STAGE);  // [2][BM + BN]: a step's e8m0 codes of each row
+  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + 2 * STAGE);  // [2][BM + BN]: a step's e8m0 codes of each row of a and of w
+  float* const scalesOf = (float*)codesOf;                                  // ... or [BM + BN] the rows' scales; behind either
+  float* const biasOf = (float*)codesOf + 2 * (BM + BN);                    // [BN]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hh = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
@@ -157,11 +152,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   // e8m0 codes: a thread fetches one row's of a step and puts them into LDS half a step later
   const int blocks = MX ? g.K / MX_BLOCK : 0;
   const int codeRow = (int)threadIdx.x < BM + BN ? (int)threadIdx.x : BM + BN - 1;
-  const uint8_t* myCodes = nullptr;
-  if constexpr(MX) {
-    if(codeRow < BM) myCodes = (const uint8_t*)g.aScales + (m0 + (codeRow < mLast ? codeRow : mLast)) * blocks;
-    else myCodes = (const uint8_t*)g.wScales + (int64_t)(n0 + (codeRow - BM < nLast ? codeRow - BM : nLast)) * blocks;
-  }
+  const bool ofA = codeRow < BM;
+  const int64_t scaleRow = ofA ? m0 + (codeRow < mLast ? codeRow : mLast) : n0 + (codeRow - BM < nLast ? codeRow - BM : nLast);
+  const uint8_t* const myCodes = (const uint8_t*)(ofA ? g.aScales : g.wScales) + scaleRow * blocks;
   unsigned fetched = 0;
   auto putCodes = [&](int step) {
     if constexpr(MX) codesOf[(step & 1) * (BM + BN) + codeRow] = shiftedCodes(fetched, blocks, step);
@@ -280,7 +273,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
     multiply(Index<1>(), 0);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr(MORE) {
-      waitLoads0();   // the next stage is there,
+      waitLoads<0>();   // the next stage is there,
       waitReads0();   // this one has been read out by this wave,
       waveBarrier();  // by all of them
       if constexpr(REQUEST != NOTHING) {
@@ -301,20 +294,25 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
     }
   };
 
+  // both stages are requested at once; what the epilogue needs and the codes come in front of them
+  const float myScale = MX ? 0.0f : ((const float*)(ofA ? g.aScales : g.wScales))[scaleRow];
+  const float myBias = ofA || g.bias == nullptr ? 0.0f : g.bias[scaleRow];
+  unsigned firstCodes = 0;
   if constexpr(MX) {
-    if(blocks >= 4) fetched = fetchCodes(myCodes, blocks, 0);
+    if(blocks >= 4) firstCodes = fetchCodes(myCodes, blocks, 0);
     else
-      for(int q = 0; q < blocks; q++) fetched |= (unsigned)myCodes[q] << (8 * (q + 4 - blocks));  // (as the shifted word)
+      for(int q = 0; q < blocks; q++) firstCodes |= (unsigned)myCodes[q] << (8 * (q + 4 - blocks));  // (as the shifted word)
+    if(steps > 1) fetched = fetchCodes(myCodes, blocks, 1);
   }
   issueAny(0);
-  putCodes(0);
-  waitLoads0();
+  if(steps > 1) issueAny(1);
+  if constexpr(!MX) scalesOf[codeRow] = myScale;
+  else codesOf[codeRow] = shiftedCodes(firstCodes, blocks, 0);
+  if(!ofA) biasOf[codeRow - BM] = myBias;
+  if(steps > 1) waitLoads<REQ_A + REQ_W>();
+  else waitLoads<0>();
   waitReads0();
   waveBarrier();
-  if(steps > 1) {
-    if constexpr(MX) fetched = fetchCodes(myCodes, blocks, 1);
-    issueAny(1);
-  }
   readCodes(0);
   readW(0, 0);
 #pragma unroll
@@ -325,38 +323,33 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   if(step + 1 < steps) body(step++, Index<1>(), Index<NOTHING>());
   body(step, Index<0>(), Index<NOTHING>());
 
-  // element v of a lane: channel 8 (v / 4) + 4 hh + v % 4 of the 32, row `col`
-  float sa[MI];
-#pragma unroll
-  for(int mi = 0; mi < MI; mi++) {
-    const int r = wm * TM + mi * 32 + col;
-    sa[mi] = MX ? 1.0f : ((const float*)g.aScales)[m0 + (r < mLast ? r : mLast)];
-  }
+  // The tile goes through LDS, so that a store instruction covers whole lines of consecutive rows. Element v of a lane: channel 8 (v / 4) + 4 hh + v % 4
+  // of the 32, row `col`; piece p of 16 bytes of row r lies at p ^ (r & 15).
+  constexpr int PER = 16 / (int)sizeof(TO), P = BN / PER;  // elements of a piece, pieces of a row
+  static_assert(BM * P * 16 <= 2 * (int)STAGE && P >= 8 && (P & (P - 1)) == 0, "the tile fits the stages");
+  constexpr int SWZ = P < 16 ? P - 1 : 15;
+  auto place = [&](int r, int p) { return lds + (unsigned)(r * P + (p ^ (r & SWZ))) * 16; };
+  waveBarrier();  // nobody reads the last stage any more
 #pragma unroll
   for(int ni = 0; ni < NI; ni++) {
     const int c0 = wn * TN + ni * 32;
     f32x4 sw[4], bias[4];
 #pragma unroll
     for(int q = 0; q < 4; q++) {
-      sw[q] = MX ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : fourFloats((const float*)g.wScales + n0, c0 + 8 * q + 4 * hh, nLast);
-      bias[q] = g.bias == nullptr ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : fourFloats(g.bias + n0, c0 + 8 * q + 4 * hh, nLast);
+      if(!MX) sw[q] = *(const f32x4*)(scalesOf + BM + c0 + 8 * q + 4 * hh);
+      bias[q] = *(const f32x4*)(biasOf + c0 + 8 * q + 4 * hh);
     }
 #pragma unroll
     for(int mi = 0; mi < MI; mi++) {
       const int r = wm * TM + mi * 32 + col;
-      TO* const row = (TO*)g.out + (m0 + r) * g.outStride + n0;
+      const float sa = MX ? 1.0f : scalesOf[r];
       u32x2 pk[4];
 #pragma unroll
       for(int q = 0; q < 4; q++) {
         f32x4 o;
 #pragma unroll
-        for(int i = 0; i < 4; i++) o[i] = acc[ni][mi][4 * q + i] * sa[mi] * sw[q][i] + bias[q][i];
-        if constexpr(OUT == DT_F32) {
-          const int c = c0 + 8 * q + 4 * hh;
-          if(r <= mLast && c + 3 <= nLast) *(f32x4u*)(row + c) = o;
-          else if(r <= mLast)
-            for(int i = 0; i < 4 && c + i <= nLast; i++) row[c + i] = o[i];
-        }
+        for(int i = 0; i < 4; i++) o[i] = (MX ? acc[ni][mi][4 * q + i] : acc[ni][mi][4 * q + i] * sa * sw[q][i]) + bias[q][i];
+        if constexpr(OUT == DT_F32) ldsWrite16(place(r, (c0 + 8 * q + 4 * hh) / 4), __builtin_bit_cast(u32x4, o));
         else {
           typename TR::V4 t;
 #pragma unroll
@@ -368,18 +361,25 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
         u32x4 whole[2];
         pairUp(pk, whole);  // whole[j]: channels 16 j + 8 hh + [0, 8)
 #pragma unroll
-        for(int j = 0; j < 2; j++) {
-          const int c = c0 + 16 * j + 8 * hh;
-          if(r <= mLast && c + 7 <= nLast) *(u32x4u*)(row + c) = whole[j];
-          else if(r <= mLast) {
-            const typename TR::V8 t = __builtin_bit_cast(typename TR::V8, whole[j]);
-#pragma unroll
-            for(int i = 0; i < 8; i++)
-              if(c + i <= nLast) row[c + i] = t[i];
-          }
-        }
+        for(int j = 0; j < 2; j++) ldsWrite16(place(r, (c0 + 16 * j + 8 * hh) / 8), whole[j]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  waitReads0();
+  waveBarrier();
+#pragma unroll 4
+  for(int at = (int)threadIdx.x; at < BM * P; at += 64 * NW) {
+    const int r = at / P, c = at % P * PER;
+    if(r > mLast || c > nLast) continue;
+    const u32x4 v = ldsRead16(place(r, at % P));
+    TO* const out = (TO*)g.out + (m0 + r) * g.outStride + n0 + c;
+    if(c + PER - 1 <= nLast) *(Out16*)out = v;
+    else {
+      struct Elements { TO e[PER]; };
+      const Elements t = __builtin_bit_cast(Elements, v);
+#pragma unroll
+      for(int i = 0; i < PER; i++)
+        if(c + i <= nLast) out[i] = t.e[i];
     }
   }
 }
@@ -388,7 +388,7 @@ template <int BM, int BN, int WM, int WN, bool MX, int OUT>
 hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const int64_t tiles = (g.rows + BM - 1) / BM * ((g.N + BN - 1) / BN);
   if(tiles > 0x7fffffff) return hipErrorInvalidValue;
-  constexpr int LDS = 2 * (BM + BN) * (KSTEP + 4);
+  constexpr int LDS = 2 * (BM + BN) * (KSTEP + 4) + BN * 4;
   auto kern = linear8Kernel<BM, BN, WM, WN, MX, OUT>;
   if(LDS > 64 * 1024) {  // opt in to the large LDS window, once per instantiation and device
     constexpr int MAX_DEVICES = 64;
