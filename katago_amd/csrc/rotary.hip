@@ -27,25 +27,7 @@ template <> struct UnalignedV<__bf16, 4> { typedef b16x4u V; };
 template <> struct UnalignedV<float, 8> { typedef f32x8u V; };
 template <> struct UnalignedV<float, 4> { typedef f32x4u V; };
 
-template <class TR, int N>
-__device__ __forceinline__ void loadN(const typename TR::T* p, float* v) {
-  if constexpr(N == 1) v[0] = TR::toFloat(p[0]);
-  else {
-    const typename UnalignedV<typename TR::T, N>::V t = *(const typename UnalignedV<typename TR::T, N>::V*)p;
-#pragma unroll
-    for(int i = 0; i < N; i++) v[i] = TR::toFloat(t[i]);
-  }
-}
-template <class TR, int N>
-__device__ __forceinline__ void storeN(typename TR::T* p, const float* v) {
-  if constexpr(N == 1) p[0] = TR::fromFloat(v[0]);
-  else {
-    typename UnalignedV<typename TR::T, N>::V t;
-#pragma unroll
-    for(int i = 0; i < N; i++) t[i] = TR::fromFloat(v[i]);
-    *(typename UnalignedV<typename TR::T, N>::V*)p = t;
-  }
-}
+template <class T> struct UnalignedV<T, 1> { typedef T V __attribute__((ext_vector_type(1))); };
 
 // sine and cosine of 2 pi t, |t| <= 1/2
 __device__ __forceinline__ void sinCosOfTurn(float t, float* s, float* c) {
@@ -59,16 +41,17 @@ __device__ __forceinline__ void sinCosOfTurn(float t, float* s, float* c) {
 
 struct RotaryLaunch {
   RotaryArgs a;
-  int hpt;                 // heads of one thread
-  int groups[2];           // ceil(heads / hpt) of q and k
-  int rotItems, copyItems; // pieces of a head: PV pairs each / PV untouched channels each
+  int perFreq[2];          // heads of q and of k that turn with one set of frequencies
+  int hpt, chunks;         // heads of one thread; such chunks of the perFreq[0] + perFreq[1] heads of a set
+  int rotItems, copyItems; // pieces of a head: PV pairs each / 2 PV untouched channels each
   unsigned token0;
   unsigned threads;
 };
 
-// A thread owns PV pairs (or PV channels to copy) of a token in hpt heads: it forms their sines and cosines once and turns head after head, HB at a
-// time so that several heads' loads are in flight. Threads of neighbouring pieces are neighbours: a head's row is read in consecutive pieces of
-// 16 bytes (16-bit types, PV = 8).
+// A thread owns PV pairs of a token in up to hpt heads of q and k that turn with the same frequencies: it forms their sines and cosines once and turns
+// head after head, HB at a time so that several heads' loads are in flight. Channels that are only copied are pieces of the same size, of the same
+// code (a lane's rotation is thrown away there). Threads of neighbouring pieces are neighbours: a head's row is read in consecutive pieces of 16
+// bytes (16-bit types, PV = 8).
 template <class TR, int PV, bool HALF>
 __global__ __launch_bounds__(256) void rotaryKernel(RotaryLaunch r) {
   typedef typename TR::T T;
@@ -76,114 +59,88 @@ __global__ __launch_bounds__(256) void rotaryKernel(RotaryLaunch r) {
   const RotaryArgs& a = r.a;
   const unsigned idx = blockIdx.x * 256u + threadIdx.x;
   if(idx >= r.threads) return;
-  const unsigned items = (unsigned)(r.rotItems + r.copyItems), groups = (unsigned)(r.groups[0] + r.groups[1]);
+  const unsigned items = (unsigned)(r.rotItems + r.copyItems), groups = (unsigned)(a.freqHeads * r.chunks);
   const unsigned item = idx % items, rest = idx / items;
   const unsigned group = rest % groups, token = rest / groups + r.token0;
   const unsigned b = token / (unsigned)a.seq, s = token % (unsigned)a.seq;
-  const int which = group < (unsigned)r.groups[0] ? 0 : 1;
-  const RotarySide& side = a.side[which];
-  const int h0 = (int)(which ? group - (unsigned)r.groups[0] : group) * r.hpt;
-  const int h1 = h0 + r.hpt < side.heads ? h0 + r.hpt : side.heads;
-  const T* const in = (const T*)side.in + b * side.inBatch + s * side.inToken;
-  T* const out = (T*)side.out + b * side.outBatch + s * side.outToken;
+  const int fh = (int)(group / (unsigned)r.chunks), first = (int)(group % (unsigned)r.chunks) * r.hpt;
+  const int all = r.perFreq[0] + r.perFreq[1], end = first + r.hpt < all ? first + r.hpt : all;  // of this set's heads: q's, then k's
+  const T* const in[2] = {(const T*)a.side[0].in + b * a.side[0].inBatch + s * a.side[0].inToken + (int64_t)fh * r.perFreq[0] * a.side[0].inHead,
+                          (const T*)a.side[1].in + b * a.side[1].inBatch + s * a.side[1].inToken + (int64_t)fh * r.perFreq[1] * a.side[1].inHead};
+  T* const out[2] = {(T*)a.side[0].out + b * a.side[0].outBatch + s * a.side[0].outToken + (int64_t)fh * r.perFreq[0] * a.side[0].outHead,
+                     (T*)a.side[1].out + b * a.side[1].outBatch + s * a.side[1].outToken + (int64_t)fh * r.perFreq[1] * a.side[1].outHead};
+  auto inOf = [&](int h) { return h < r.perFreq[0] ? in[0] + h * a.side[0].inHead : in[1] + (h - r.perFreq[0]) * a.side[1].inHead; };
+  auto outOf = [&](int h) { return h < r.perFreq[0] ? out[0] + h * a.side[0].outHead : out[1] + (h - r.perFreq[0]) * a.side[1].outHead; };
 
-  if(item >= (unsigned)r.rotItems) {  // channels that are not turned (only where out is another buffer)
-    const int c = 2 * a.pairs + (int)(item - (unsigned)r.rotItems) * PV;
-    for(int h = h0; h < h1; h++) {
-      const T* const ip = in + h * side.inHead + c;
-      T* const op = out + h * side.outHead + c;
-      if(c + PV <= a.headDim) {
-        float v[PV];
-        loadN<TR, PV>(ip, v);
-        storeN<TR, PV>(op, v);
-      }
-      else
-        for(int i = 0; c + i < a.headDim; i++) op[i] = ip[i];
+  const bool copied = item >= (unsigned)r.rotItems;
+  const int c = 2 * a.pairs + (int)(item - (unsigned)r.rotItems) * 2 * PV;  // of a copied piece
+  if(copied && c + 2 * PV > a.headDim) {  // the last channels of a head, fewer than a piece
+    for(int h = first; h < end; h++) {
+      const T* const ip = inOf(h);
+      T* const op = outOf(h);
+      for(int i = c; i < a.headDim; i++) op[i] = ip[i];
     }
     return;
   }
+  const int p0 = copied ? 0 : (int)item * PV;  // pairs is a multiple of PV
+  const int at0 = copied ? c : HALF ? p0 : 2 * p0, at1 = copied || !HALF ? at0 + PV : p0 + a.pairs;
 
-  const int p0 = (int)item * PV;  // pairs is a multiple of PV
+  typedef typename UnalignedV<T, PV>::V V;
+  V u[HB], v[HB];  // channels at0 + [0, PV) and at1 + [0, PV) of a head
+  auto fetch = [&](int hb) {
+#pragma unroll
+    for(int j = 0; j < HB; j++) {
+      if(hb + j >= end) break;
+      const T* const ip = inOf(hb + j);
+      u[j] = *(const V*)(ip + at0);
+      v[j] = *(const V*)(ip + at1);
+    }
+  };
+  fetch(first);
+
   double pos[2] = {0.0, 0.0};
   for(int ax = 0; ax < a.axes; ax++) {
     const int64_t at = b * a.posBatch + s * a.posToken + ax * a.posAxis;
     pos[ax] = a.pos64 ? (double)((const int64_t*)a.positions)[at] : (double)((const int32_t*)a.positions)[at];
   }
   float cs[PV], sn[PV];
-  int turned = -1;  // the frequencies' head that cs / sn belong to
-  const int perFreq = side.heads / a.freqHeads;
-  for(int hb = h0; hb < h1; hb += HB) {
-    float u[HB][PV], v[HB][PV];
+  const double* const f = a.freqs + (size_t)fh * a.axes * a.pairs + p0;
+#pragma unroll
+  for(int i = 0; i < PV; i++) {
+    double t = pos[0] * f[i];
+    if(a.axes == 2) t += pos[1] * f[a.pairs + i];
+    t *= 0.15915494309189533577;  // 1 / 2 pi
+    float sv, cv;
+    sinCosOfTurn((float)(t - __builtin_rint(t)), &sv, &cv);
+    cs[i] = cv * a.magnitude;
+    sn[i] = (a.inverse ? -sv : sv) * a.magnitude;
+  }
+
+  for(int hb = first; hb < end; hb += HB) {
+    if(hb != first) fetch(hb);
 #pragma unroll
     for(int j = 0; j < HB; j++) {
-      if(hb + j >= h1) break;
-      const T* const ip = in + (hb + j) * side.inHead;
-      if(HALF) {
-        loadN<TR, PV>(ip + p0, u[j]);
-        loadN<TR, PV>(ip + a.pairs + p0, v[j]);
-      }
-      else {
-        float w[2 * PV];
-        if constexpr(PV == 1) {
-          w[0] = TR::toFloat(ip[2 * p0]);
-          w[1] = TR::toFloat(ip[2 * p0 + 1]);
+      if(hb + j >= end) break;
+      V x, y;
+#pragma unroll
+      for(int i = 0; i < PV; i++) {  // pair i: HALF (u[i], v[i]), else neighbours of u and v in a row
+        const float m = TR::toFloat(HALF ? u[j][i] : 2 * i < PV ? u[j][(2 * i) % PV] : v[j][(2 * i) % PV]);
+        const float n = TR::toFloat(HALF ? v[j][i] : 2 * i + 1 < PV ? u[j][(2 * i + 1) % PV] : v[j][(2 * i + 1) % PV]);
+        const T p = TR::fromFloat(m * cs[i] - n * sn[i]), q = TR::fromFloat(m * sn[i] + n * cs[i]);
+        if(HALF) {
+          x[i] = p;
+          y[i] = q;
         }
         else {
-          loadN<TR, PV>(ip + 2 * p0, w);
-          loadN<TR, PV>(ip + 2 * p0 + PV, w + PV);
-        }
-#pragma unroll
-        for(int i = 0; i < PV; i++) {
-          u[j][i] = w[2 * i];
-          v[j][i] = w[2 * i + 1];
+          if(2 * i < PV) x[(2 * i) % PV] = p;
+          else y[(2 * i) % PV] = p;
+          if(2 * i + 1 < PV) x[(2 * i + 1) % PV] = q;
+          else y[(2 * i + 1) % PV] = q;
         }
       }
-    }
-#pragma unroll
-    for(int j = 0; j < HB; j++) {
-      if(hb + j >= h1) break;
-      const int fh = (hb + j) / perFreq;
-      if(fh != turned) {
-        turned = fh;
-        const double* const f = a.freqs + (size_t)fh * a.axes * a.pairs + p0;
-#pragma unroll
-        for(int i = 0; i < PV; i++) {
-          double t = pos[0] * f[i];
-          if(a.axes == 2) t += pos[1] * f[a.pairs + i];
-          t *= 0.15915494309189533577;  // 1 / 2 pi
-          float sv, cv;
-          sinCosOfTurn((float)(t - __builtin_rint(t)), &sv, &cv);
-          cs[i] = cv * a.magnitude;
-          sn[i] = (a.inverse ? -sv : sv) * a.magnitude;
-        }
-      }
-      float x[PV], y[PV];
-#pragma unroll
-      for(int i = 0; i < PV; i++) {
-        x[i] = u[j][i] * cs[i] - v[j][i] * sn[i];
-        y[i] = u[j][i] * sn[i] + v[j][i] * cs[i];
-      }
-      T* const op = out + (hb + j) * side.outHead;
-      if(HALF) {
-        storeN<TR, PV>(op + p0, x);
-        storeN<TR, PV>(op + a.pairs + p0, y);
-      }
-      else {
-        float w[2 * PV];
-#pragma unroll
-        for(int i = 0; i < PV; i++) {
-          w[2 * i] = x[i];
-          w[2 * i + 1] = y[i];
-        }
-        if constexpr(PV == 1) {
-          op[2 * p0] = TR::fromFloat(w[0]);
-          op[2 * p0 + 1] = TR::fromFloat(w[1]);
-        }
-        else {
-          storeN<TR, PV>(op + 2 * p0, w);
-          storeN<TR, PV>(op + 2 * p0 + PV, w + PV);
-        }
-      }
+      T* const op = outOf(hb + j);
+      *(V*)(op + at0) = copied ? u[j] : x;
+      *(V*)(op + at1) = copied ? v[j] : y;
     }
   }
 }
@@ -192,14 +149,18 @@ template <class TR, int PV, bool HALF>
 hipError_t launchPieces(const RotaryArgs& a, hipStream_t stream) {
   RotaryLaunch r;
   r.a = a;
+  for(int i = 0; i < 2; i++) r.perFreq[i] = a.side[i].heads / a.freqHeads;
   r.rotItems = a.pairs / PV;
-  const bool copies = (a.side[0].heads > 0 && a.side[0].in != a.side[0].out) || (a.side[1].heads > 0 && a.side[1].in != a.side[1].out);
-  r.copyItems = copies ? (a.headDim - 2 * a.pairs + PV - 1) / PV : 0;
-  const int items = r.rotItems + r.copyItems;
+  const bool copies = a.side[0].in != a.side[0].out || (a.side[1].heads > 0 && a.side[1].in != a.side[1].out);
+  r.copyItems = copies ? (a.headDim - 2 * a.pairs + 2 * PV - 1) / (2 * PV) : 0;
+  const int items = r.rotItems + r.copyItems, all = r.perFreq[0] + r.perFreq[1];
+  // Few tokens: one head a thread, all loads of the call in flight at once (8 tokens, 32 + 8 heads of 128: 5.6 us with 8 heads a thread). Many: 8
+  // heads share a thread's sines and cosines, once there are threads enough to fill the chip.
   r.hpt = 8;
-  r.groups[0] = (a.side[0].heads + r.hpt - 1) / r.hpt;
-  r.groups[1] = (a.side[1].heads + r.hpt - 1) / r.hpt;
-  const int64_t perToken = (int64_t)items * (r.groups[0] + r.groups[1]);
+  while(r.hpt > 1 && a.tokens * items * a.freqHeads * ((all + r.hpt - 1) / r.hpt) < 256 * 1024) r.hpt /= 2;
+  r.chunks = (all + r.hpt - 1) / r.hpt;
+  r.hpt = (all + r.chunks - 1) / r.chunks;  // evenly
+  const int64_t perToken = (int64_t)items * a.freqHeads * r.chunks;
   const int64_t most = (int64_t)0x7fffffff / perToken;  // tokens of one launch: its threads are counted in 31 bits
   for(int64_t t0 = 0; t0 < a.tokens; t0 += most) {
     const int64_t n = a.tokens - t0 < most ? a.tokens - t0 : most;
@@ -214,7 +175,8 @@ hipError_t launchPieces(const RotaryArgs& a, hipStream_t stream) {
 }
 template <class TR>
 hipError_t launchType(const RotaryArgs& a, hipStream_t stream) {
-  if(a.pairs % 8 == 0) return a.half ? launchPieces<TR, 8, true>(a, stream) : launchPieces<TR, 8, false>(a, stream);
+  // pieces of 16 bytes: 8 pairs of a 16-bit type, 4 of fp32 (8 of fp32 take 184 registers: 4 x 8191 x 9 heads of 64 in 34 us against 28)
+  if(sizeof(typename TR::T) == 2 && a.pairs % 8 == 0) return a.half ? launchPieces<TR, 8, true>(a, stream) : launchPieces<TR, 8, false>(a, stream);
   if(a.pairs % 4 == 0) return a.half ? launchPieces<TR, 4, true>(a, stream) : launchPieces<TR, 4, false>(a, stream);
   return a.half ? launchPieces<TR, 1, true>(a, stream) : launchPieces<TR, 1, false>(a, stream);
 }
