@@ -33,8 +33,11 @@ void aligned(const char* entry, const char* name, const void* p, size_t to) {
 class OnDevice {
  public:
   explicit OnDevice(int device) {
-    int n = 0;
-    if(hipGetDeviceCount(&n) != hipSuccess || n <= 0) throw Error(KMX_ERR_DEVICE, "no usable HIP device (katamx has no CPU fallback)");
+    static const int n = [] {
+      int c = 0;
+      return hipGetDeviceCount(&c) == hipSuccess ? c : 0;
+    }();
+    if(n <= 0) throw Error(KMX_ERR_DEVICE, "no usable HIP device (katamx has no CPU fallback)");
     if(device < 0 || device >= n) throw Error(KMX_ERR_INVALID_ARG, "there is no device " + std::to_string(device));
     hipCheck(hipGetDevice(&before_), "hipGetDevice");
     if(before_ != device) {

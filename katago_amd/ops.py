@@ -24,7 +24,6 @@ MX_BLOCK = 32
 E4M3_MAX = 448.0
 _TYPES = {torch.float16: capi.PREC_FP16, torch.bfloat16: capi.PREC_BF16, torch.float32: capi.PREC_FP32}
 _CODES = torch.float8_e4m3fn
-_SCALE_TYPE = {"row": torch.float32, "mx": torch.float8_e8m0fnu}
 
 Normed = collections.namedtuple("Normed", ["sum", "y", "codes", "scales"])
 
@@ -44,23 +43,29 @@ def _refuse(why):
     raise KatamxError(capi.KMX_ERR_INVALID_ARG, why)
 
 
-def _on_device(*tensors):
-    """The device all of them are on; gradients are refused."""
-    device = None
-    for name, t in tensors:
+def _on_device(names, *tensors):
+    """The index of the device all of them are on (None among them: not given); gradients are refused."""
+    index, grad = None, torch.is_grad_enabled()
+    for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor):
-            _refuse("%s must be a tensor" % name)
-        if t.device.type != "cuda":
-            _refuse("%s is on %s: the operators work on device tensors" % (name, t.device))
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            _refuse("%s is on %s, the others on %s" % (name, t.device, device))
-        if t.requires_grad and torch.is_grad_enabled():
-            _refuse("%s requires a gradient and the operators compute none: call them under torch.no_grad()" % name)
-    return device
+        try:
+            d = t.get_device()
+        except AttributeError:
+            _refuse("%s must be a tensor" % _name(names, tensors, t))
+        if d != index:
+            if d < 0 or not t.is_cuda:
+                _refuse("%s is on %s: the operators work on device tensors" % (_name(names, tensors, t), t.device))
+            if index is not None:
+                _refuse("%s is on device %d, the others on %d" % (_name(names, tensors, t), d, index))
+            index = d
+        if grad and t.requires_grad:
+            _refuse("%s requires a gradient and the operators compute none: call them under torch.no_grad()" % _name(names, tensors, t))
+    return index
+
+
+def _name(names, tensors, t):
+    return names.split()[[u is t for u in tensors].index(True)]
 
 
 def _rows(name, t, channels=None):
@@ -97,22 +102,25 @@ def _vector(name, t, length):
     return t.data_ptr()
 
 
-def _output(name, given, shape, dtype, device):
-    if given is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if given.dtype != dtype or tuple(given.shape) != tuple(shape):
+def _given(name, t, shape, dtype):
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
         _refuse("%s must be %s of shape %s" % (name, dtype, tuple(shape)))
-    return given
+    return t
 
 
-def _type(name, t):
-    if t.dtype not in _TYPES:
-        _refuse("%s is %s, not float16, bfloat16 or float32" % (name, t.dtype))
-    return _TYPES[t.dtype]
+def _type(name, dtype):
+    typ = _TYPES.get(dtype)
+    if typ is None:
+        _refuse("%s is %s, not float16, bfloat16 or float32" % (name, dtype))
+    return typ
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _current_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# (the same address without a Stream object around it, which costs 2 us of a call's 10)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
 def rms_norm(x, weight=None, eps=1e-6, *, beta=None, residual=None, mask=None, scales=None, want_y=None, sum_out=None, y_out=None):
@@ -124,62 +132,64 @@ def rms_norm(x, weight=None, eps=1e-6, *, beta=None, residual=None, mask=None, s
 
     want_y: whether y itself is returned (by default only without scales). weight and beta: float32 [channels]. sum_out / y_out: the tensors to write,
     each may be x or residual itself. Returns Normed(sum, y, codes, scales), None for what was not asked for."""
-    device = _on_device(("x", x), ("weight", weight), ("beta", beta), ("residual", residual), ("mask", mask), ("sum_out", sum_out), ("y_out", y_out))
-    typ = _type("x", x)
-    if scales not in SCALES:
+    device = _on_device("x weight beta residual mask sum_out y_out", x, weight, beta, residual, mask, sum_out, y_out)
+    dtype = x.dtype
+    a = capi.RmsNormArgs(_type("x", dtype), SCALES.get(scales, -1))
+    if a.scale_kind < 0:
         _refuse("scales must be None, 'row' or 'mx'")
     if want_y is None:
         want_y = scales is None or y_out is not None
     if y_out is not None and not want_y or sum_out is not None and residual is None:
         _refuse("an output is given that is not computed")
     shape = x.shape
-    rows, c, xs = _rows("x", x)
-    if scales == "mx" and c % MX_BLOCK:
-        _refuse("scales for 32 channels each need a multiple of 32 channels, not %d" % c)
-    a = capi.RmsNormArgs()
-    a.type, a.scale_kind, a.rows, a.channels, a.epsilon = typ, SCALES[scales], rows, c, eps
-    a.x, a.x_stride = x.data_ptr(), xs
+    rows, c, a.x_stride = _rows("x", x)
+    a.rows, a.channels, a.epsilon, a.x = rows, c, eps, x.data_ptr()
     a.weight, a.beta, a.mask = _vector("weight", weight, c), _vector("beta", beta, c), _vector("mask", mask, rows)
-    total = None
+    total = y = codes = sc = None
     if residual is not None:
-        if residual.dtype != x.dtype or residual.shape != shape:
+        if residual.dtype != dtype or residual.shape != shape:
             _refuse("residual must be of x's type and shape")
-        total = _output("sum_out", sum_out, shape, x.dtype, device)
         a.residual, a.residual_stride = residual.data_ptr(), _rows("residual", residual)[2]
+        total = torch.empty_like(x) if sum_out is None else _given("sum_out", sum_out, shape, dtype)
         a.sum, a.sum_stride = total.data_ptr(), _rows("sum_out", total)[2]
-    y = None
     if want_y:
-        y = _output("y_out", y_out, shape, x.dtype, device)
+        y = torch.empty_like(x) if y_out is None else _given("y_out", y_out, shape, dtype)
         a.y, a.y_stride = y.data_ptr(), _rows("y_out", y)[2]
-    codes = sc = None
     if scales is not None:
-        codes, sc = _codes_for(shape, scales, device)
+        codes, sc = _codes_for(x, scales)
         a.codes, a.codes_stride, a.scales = codes.data_ptr(), c, sc.data_ptr()
     if rows:
-        lib = _library()
-        capi.check(lib.kmx_rmsnorm(device.index, _stream(device), ctypes.byref(a)), lib)
+        lib = _lib or _library()
+        rc = lib.kmx_rmsnorm(device, _stream(device), ctypes.byref(a))
+        if rc:
+            capi.check(rc, lib)
     return Normed(total, y, codes, sc)
 
 
-def _codes_for(shape, scales, device):
-    codes = torch.empty(shape, dtype=_CODES, device=device)
-    sshape = tuple(shape[:-1]) if scales == "row" else tuple(shape[:-1]) + (shape[-1] // MX_BLOCK,)
-    return codes, torch.empty(sshape, dtype=_SCALE_TYPE[scales], device=device)
+def _codes_for(x, scales):
+    shape = x.shape
+    if scales == "row":
+        sc = x.new_empty(shape[:-1], dtype=torch.float32)
+    else:
+        if shape[-1] % MX_BLOCK:
+            _refuse("scales for 32 channels each need a multiple of 32 channels, not %d" % shape[-1])
+        sc = x.new_empty(shape[:-1] + (shape[-1] // MX_BLOCK,), dtype=torch.float8_e8m0fnu)
+    return x.new_empty(shape, dtype=_CODES), sc
 
 
 def quantize(x, scales="row"):
     """(codes, scales) of x's rows ([..., channels]) in e4m3: what linear8 multiplies. scales as in rms_norm."""
-    device = _on_device(("x", x))
-    typ = _type("x", x)
+    device = _on_device("x", x)
+    typ = _type("x", x.dtype)
     if scales not in ("row", "mx"):
         _refuse("scales must be 'row' or 'mx'")
     rows, c, xs = _rows("x", x)
-    if scales == "mx" and c % MX_BLOCK:
-        _refuse("scales for 32 channels each need a multiple of 32 channels, not %d" % c)
-    codes, sc = _codes_for(x.shape, scales, device)
+    codes, sc = _codes_for(x, scales)
     if rows:
-        lib = _library()
-        capi.check(lib.kmx_quantize(device.index, _stream(device), typ, SCALES[scales], rows, c, x.data_ptr(), xs, codes.data_ptr(), c, sc.data_ptr()), lib)
+        lib = _lib or _library()
+        rc = lib.kmx_quantize(device, _stream(device), typ, SCALES[scales], rows, c, x.data_ptr(), xs, codes.data_ptr(), c, sc.data_ptr())
+        if rc:
+            capi.check(rc, lib)
     return codes, sc
 
 
@@ -199,7 +209,7 @@ def linear8(codes, scales, weight_codes, weight_scales, bias=None, *, out_dtype=
     """[..., n] = (codes * scales) (weight_codes * weight_scales)^T + bias: codes e4m3 [..., k], weight_codes e4m3 [n, k], scales of both as
     rms_norm / quantize return them (of one kind), bias float32 [n]. k is a multiple of 16 (mx: 32). out_dtype float16, bfloat16 or float32; float32
     is summed in fp32 throughout, the others on the 8-bit matrix instructions (katamx_ops.h)."""
-    device = _on_device(("codes", codes), ("scales", scales), ("weight_codes", weight_codes), ("weight_scales", weight_scales), ("bias", bias), ("out", out))
+    device = _on_device("codes scales weight_codes weight_scales bias out", codes, scales, weight_codes, weight_scales, bias, out)
     if weight_codes.dim() != 2:
         _refuse("weight_codes must be [n, k]")
     n, k, ws = _rows("weight_codes", weight_codes)
@@ -207,28 +217,28 @@ def linear8(codes, scales, weight_codes, weight_scales, bias=None, *, out_dtype=
     kind = _kind_of("codes", codes, scales, rows, k)
     if _kind_of("weight_codes", weight_codes, weight_scales, n, k) != kind:
         _refuse("the scales of codes and weight_codes are of different kinds")
-    if out is not None:
-        out_dtype = out.dtype
-    if out_dtype not in _TYPES:
-        _refuse("out_dtype is %s, not float16, bfloat16 or float32" % out_dtype)
-    out = _output("out", out, tuple(codes.shape[:-1]) + (n,), out_dtype, device)
-    a = capi.Linear8Args()
-    a.out_type, a.scale_kind, a.rows, a.n, a.k = _TYPES[out_dtype], kind, rows, n, k
-    a.a, a.a_scales, a.w, a.w_scales, a.out = codes.data_ptr(), scales.data_ptr(), weight_codes.data_ptr(), weight_scales.data_ptr(), out.data_ptr()
-    a.bias = _vector("bias", bias, n)
-    a.a_stride, a.w_stride, a.out_stride = (cs if rows > 1 else k), (ws if n > 1 else k), _rows("out", out)[2]
+    shape = codes.shape[:-1] + (n,)
+    if out is None:
+        typ = _type("out_dtype", out_dtype)
+        out = codes.new_empty(shape, dtype=out_dtype)
+        stride = n
+    else:
+        typ = _type("out", out.dtype)
+        stride = _rows("out", _given("out", out, shape, out.dtype))[2]
     if rows:
-        lib = _library()
-        capi.check(lib.kmx_linear8(device.index, _stream(device), ctypes.byref(a)), lib)
+        a = capi.Linear8Args(typ, kind, rows, n, k, codes.data_ptr(), scales.data_ptr(), weight_codes.data_ptr(), weight_scales.data_ptr(),
+                             _vector("bias", bias, n), out.data_ptr(), cs, ws, stride)
+        lib = _lib or _library()
+        rc = lib.kmx_linear8(device, _stream(device), ctypes.byref(a))
+        if rc:
+            capi.check(rc, lib)
     return out
 
 
 def _token_strides(name, t, lead):
     """(batch, seq, head) strides of [batch, seq, heads, dim] or [tokens, heads, dim]"""
-    if t.dim() != lead + 2:
-        _refuse("%s must be [batch, seq, heads, head_dim] or [tokens, heads, head_dim], as the others" % name)
     st = t.stride()
-    if t.shape[-1] > 1 and st[-1] != 1:
+    if st[-1] != 1 and t.shape[-1] > 1:
         _refuse("%s: channels must be contiguous" % name)
     return (st[0] if lead == 2 else 0), st[lead - 1], st[lead]
 
@@ -242,8 +252,8 @@ def rotary(q, k, positions, frequencies, *, layout="interleaved", magnitude=1.0,
     left out where there is one. frequencies: float64 [pairs], [axes, pairs] or [freq_heads, axes, pairs] on the device (rotary_frequencies(),
     board_frequencies()); freq_heads divides the heads of q and of k: query heads turn as the key head they read. inverse: the turn back, and
     the transpose. q_out / k_out: the tensors to write, each may be q / k itself. Returns (q_out, k_out)."""
-    device = _on_device(("q", q), ("k", k), ("positions", positions), ("frequencies", frequencies), ("q_out", q_out), ("k_out", k_out))
-    typ = _type("q", q)
+    device = _on_device("q k positions frequencies q_out k_out", q, k, positions, frequencies, q_out, k_out)
+    typ = _type("q", q.dtype)
     if layout not in ("interleaved", "half"):
         _refuse("layout must be 'interleaved' or 'half'")
     lead = q.dim() - 2
@@ -267,26 +277,27 @@ def rotary(q, k, positions, frequencies, *, layout="interleaved", magnitude=1.0,
     if pshape not in wanted:
         _refuse("positions must be one for each token: %s for q's %s" % (tuple(positions.shape), tuple(q.shape)))
     pos_batch, pos_seq = pst if len(pshape) == 2 else (0, pst[0])
-    a = capi.RotaryArgs()
-    a.type, a.half, a.inverse, a.magnitude = typ, int(layout == "half"), int(bool(inverse)), magnitude
-    a.batch, a.seq, a.q_heads, a.head_dim, a.pairs, a.axes, a.freq_heads = batch, seq, heads, dim, fshape[2], axes, fshape[0]
-    a.frequencies, a.positions, a.positions_are_64bit = frequencies.data_ptr(), positions.data_ptr(), int(positions.dtype == torch.int64)
-    a.pos_batch_stride, a.pos_seq_stride, a.pos_axis_stride = pos_batch, pos_seq, pos_axis
-    q_out = _output("q_out", q_out, q.shape, q.dtype, device)
-    a.q = capi.RotaryTensor(q.data_ptr(), q_out.data_ptr(), *_token_strides("q", q, lead), *_token_strides("q_out", q_out, lead))
+    k_heads = 0
     if k is not None:
-        if k.dtype != q.dtype or k.dim() != q.dim() or k.shape[:lead] != q.shape[:lead] or k.shape[-1] != dim:
+        if k.dtype != q.dtype or k.dim() != lead + 2 or k.shape[:lead] != q.shape[:lead] or k.shape[-1] != dim:
             _refuse("k must have q's type, tokens and head_dim")
-        a.k_heads = k.shape[lead]
-        k_out = _output("k_out", k_out, k.shape, k.dtype, device)
-        a.k = capi.RotaryTensor(k.data_ptr(), k_out.data_ptr(), *_token_strides("k", k, lead), *_token_strides("k_out", k_out, lead))
+        k_heads = k.shape[lead]
     elif k_out is not None:
         _refuse("an output is given that is not computed")
-    if batch * seq and heads and (k is None or a.k_heads):
-        lib = _library()
-        capi.check(lib.kmx_rotary(device.index, _stream(device), ctypes.byref(a)), lib)
-    elif not heads or (k is not None and not a.k_heads):
+    if not heads or (k is not None and not k_heads):
         _refuse("q and k must have heads")
+    q_out = torch.empty_like(q) if q_out is None else _given("q_out", q_out, q.shape, q.dtype)
+    tensors = [capi.RotaryTensor(q.data_ptr(), q_out.data_ptr(), *_token_strides("q", q, lead), *_token_strides("q_out", q_out, lead))]
+    if k is not None:
+        k_out = torch.empty_like(k) if k_out is None else _given("k_out", k_out, k.shape, k.dtype)
+        tensors.append(capi.RotaryTensor(k.data_ptr(), k_out.data_ptr(), *_token_strides("k", k, lead), *_token_strides("k_out", k_out, lead)))
+    if batch * seq:
+        a = capi.RotaryArgs(typ, layout == "half", bool(inverse), magnitude, batch, seq, heads, k_heads, dim, fshape[2], axes, fshape[0],
+                            frequencies.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, pos_batch, pos_seq, pos_axis, *tensors)
+        lib = _lib or _library()
+        rc = lib.kmx_rotary(device, _stream(device), ctypes.byref(a))
+        if rc:
+            capi.check(rc, lib)
     return q_out, k_out
 
 
