@@ -384,6 +384,133 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   }
 }
 
+// Few rows: the time is the weights' way from memory, so they go straight into registers, every byte requested at once. A work-group owns 16 output
+// channels and up to 16 MT rows; its 8 waves take every eighth step of 128 k (v_mfma_scale_f32_16x16x128_f8f6f4, or four of 16x16x32_bf16) and add their
+// sums in LDS, in the order of the waves. Lane (r = l % 16, part = l / 16) holds k 16 part + [0, 16) and 64 + 16 part + [0, 16) of row r: 128
+// consecutive bytes of each weight row a step; the e8m0 code of block b comes from the lanes of part b.
+template <int MT, bool MX, int OUT>
+__global__ __launch_bounds__(512) void linear8FewKernel(Linear8Args g) {
+  typedef typename OutTraits<OUT>::TR TR;
+  typedef typename TR::T TO;
+  constexpr bool EXACT = OUT == DT_F32;
+  constexpr int NW = 8, DEPTH = MT == 1 ? 4 : 2;  // waves; steps whose requests are in flight
+  __shared__ float sums[NW][16][MT * 16 + 4];     // [wave][channel][row]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, part = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16;
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  const int nLast = (g.N - n0 < 16 ? g.N - n0 : 16) - 1, mLast = (int)(g.rows - m0 < 16 * MT ? g.rows - m0 : 16 * MT) - 1;
+  const int pieces = g.K / 16, steps = (g.K + KSTEP - 1) / KSTEP, blocks = MX ? g.K / MX_BLOCK : 0;
+  const int wRow = n0 + (col < nLast ? col : nLast);
+  const uint8_t* const wp = g.w + (int64_t)wRow * g.wStride;
+  const uint8_t* const wc = MX ? (const uint8_t*)g.wScales + (int64_t)wRow * blocks : nullptr;
+  const uint8_t* ap[MT];
+  const uint8_t* ac[MT];
+#pragma unroll
+  for(int mt = 0; mt < MT; mt++) {
+    const int64_t row = m0 + (mt * 16 + col < mLast ? mt * 16 + col : mLast);
+    ap[mt] = g.a + row * g.aStride;
+    ac[mt] = MX ? (const uint8_t*)g.aScales + row * blocks : nullptr;
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for(int mt = 0; mt < MT; mt++)
+#pragma unroll
+    for(int v = 0; v < 4; v++) acc[mt][v] = 0.0f;
+
+  for(int s0 = wave; s0 < steps; s0 += NW * DEPTH) {
+    u32x4 fw[DEPTH][2], fa[DEPTH][MT][2];
+    unsigned cw[DEPTH], ca[DEPTH][MT];
+#pragma unroll
+    for(int d = 0; d < DEPTH; d++) {  // steps beyond the last: its pieces again, not multiplied
+      const int step = s0 + d * NW < steps ? s0 + d * NW : steps - 1;
+#pragma unroll
+      for(int b = 0; b < 2; b++) {  // pieces beyond K: the row's last one, the weights' then zeroed
+        const int want = step * KPIECES + 4 * b + part, piece = want < pieces ? want : pieces - 1;
+        fw[d][b] = *(const u32x4*)(wp + (size_t)piece * 16);
+#pragma unroll
+        for(int mt = 0; mt < MT; mt++) fa[d][mt][b] = *(const u32x4*)(ap[mt] + (size_t)piece * 16);
+      }
+      if constexpr(MX) {
+        if(blocks >= 4) {
+          cw[d] = fetchCodes(wc, blocks, step);
+#pragma unroll
+          for(int mt = 0; mt < MT; mt++) ca[d][mt] = fetchCodes(ac[mt], blocks, step);
+        }
+        else {  // (as the words that shiftedCodes takes; one step)
+          cw[d] = 0;
+#pragma unroll
+          for(int mt = 0; mt < MT; mt++) ca[d][mt] = 0;
+          for(int q = 0; q < blocks; q++) {
+            cw[d] |= (unsigned)wc[q] << (8 * (q + 4 - blocks));
+#pragma unroll
+            for(int mt = 0; mt < MT; mt++) ca[d][mt] |= (unsigned)ac[mt][q] << (8 * (q + 4 - blocks));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for(int d = 0; d < DEPTH; d++) {
+      const int step = s0 + d * NW;
+      if(step >= steps) break;
+#pragma unroll
+      for(int b = 0; b < 2; b++)
+        if(step * KPIECES + 4 * b + part >= pieces) {
+#pragma unroll
+          for(int i = 0; i < 4; i++) fw[d][b][i] = 0;
+        }
+      if constexpr(MX) {
+        cw[d] = shiftedCodes(cw[d], blocks, step);
+#pragma unroll
+        for(int mt = 0; mt < MT; mt++) ca[d][mt] = shiftedCodes(ca[d][mt], blocks, step);
+      }
+#pragma unroll
+      for(int mt = 0; mt < MT; mt++) {
+        if constexpr(EXACT) {
+#pragma unroll
+          for(int q = 0; q < 4; q++) {  // 8 codes of each lane
+            const int b = q >> 1, e = 2 * (q & 1), shift = 8 * (2 * b + (part >> 1));
+            acc[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16Of(fw[d][b][e], fw[d][b][e + 1], MX ? ofE8m0(cw[d] >> shift & 255u) : 1.0f),
+                                                              bf16Of(fa[d][mt][b][e], fa[d][mt][b][e + 1], MX ? ofE8m0(ca[d][mt] >> shift & 255u) : 1.0f), acc[mt], 0, 0, 0);
+          }
+        }
+        else {
+          i32x8 xw, xa;
+#pragma unroll
+          for(int i = 0; i < 8; i++) {
+            xw[i] = (int)fw[d][i >> 2][i & 3];
+            xa[i] = (int)fa[d][mt][i >> 2][i & 3];
+          }
+          constexpr int UNIT = 0x7f7f7f7f;
+          acc[mt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xw, xa, acc[mt], 0, 0, 0, MX ? (int)(cw[d] >> (8 * part)) : UNIT, 0,
+                                                                     MX ? (int)(ca[d][mt] >> (8 * part)) : UNIT);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for(int mt = 0; mt < MT; mt++)  // element v of a lane: channel 4 part + v, row `col`
+#pragma unroll
+    for(int v = 0; v < 4; v++) sums[wave][4 * part + v][mt * 16 + col] = acc[mt][v];
+  __syncthreads();
+  for(int at = (int)threadIdx.x; at < MT * 16 * 16; at += 64 * NW) {
+    const int c = at & 15, r = at >> 4;
+    if(r > mLast || c > nLast) continue;
+    float x = 0.0f;
+#pragma unroll
+    for(int w = 0; w < NW; w++) x += sums[w][c][r];
+    if(!MX) x = x * ((const float*)g.aScales)[m0 + r] * ((const float*)g.wScales)[n0 + c];
+    if(g.bias != nullptr) x += g.bias[n0 + c];
+    ((TO*)g.out)[(m0 + r) * g.outStride + n0 + c] = TR::fromFloat(x);
+  }
+}
+
+template <int MT, bool MX, int OUT>
+hipError_t launchFew(const Linear8Args& g, hipStream_t stream) {
+  auto kern = linear8FewKernel<MT, MX, OUT>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((g.N + 15) / 16), (unsigned)((g.rows + 16 * MT - 1) / (16 * MT))), dim3(512), 0, stream, g);
+  return hipGetLastError();
+}
 template <int BM, int BN, int WM, int WN, bool MX, int OUT>
 hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const int64_t tiles = (g.rows + BM - 1) / BM * ((g.N + BN - 1) / BN);
@@ -408,6 +535,9 @@ hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
 }
 template <bool MX, int OUT>
 hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
+  if(g.rows <= 16) return launchFew<1, MX, OUT>(g, stream);
+  if(g.rows <= 32) return launchFew<2, MX, OUT>(g, stream);
+  if(g.rows <= 64) return launchFew<4, MX, OUT>(g, stream);
   auto tiles = [&](int bm, int bn) { return (g.rows + bm - 1) / bm * ((g.N + bn - 1) / bn); };
   if constexpr(OUT != DT_F32)
     if(tiles(256, 256) >= 256) return launchTile<256, 256, 2, 4, MX, OUT>(g, stream);

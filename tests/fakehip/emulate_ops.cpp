@@ -80,10 +80,70 @@ inline F16 mfmaScale(I8 a, I8 b, F16 c, int sa, int sb) {
   }
   return c;
 }
+// v_mfma_scale_f32_16x16x128_f8f6f4 on e4m3: lane (row or column l % 16, part l / 16) holds k = 16 part + [0, 16) and 64 + 16 part + [0, 16); the scale of
+// k 32 b + [0, 32) is that of part b. C element v of a lane: row 4 part + v, column l % 16.
+template <class I8, class F4>
+inline F4 mfmaScale16(I8 a, I8 b, F4 c, int sa, int sb) {
+  Wave& w = cur->waves[tIdx.x >> 6];
+  const unsigned lane = tIdx.x & 63;
+  uint8_t av[64][32], bv[64][32];
+  int as[64], bs[64];
+  {
+    const unsigned set = waveOp++ & 1;
+    memcpy(&w.opA[set][lane][0], &a, 32);
+    memcpy(&w.opB[set][lane][0], &b, 32);
+    w.bar->arrive_and_wait();
+    memcpy(av, w.opA[set], sizeof(av));
+    memcpy(bv, w.opB[set], sizeof(bv));
+  }
+  {
+    const unsigned set = waveOp++ & 1;
+    memcpy(&w.opA[set][lane][0], &sa, 4);
+    memcpy(&w.opB[set][lane][0], &sb, 4);
+    w.bar->arrive_and_wait();
+    for(int l = 0; l < 64; l++) {
+      memcpy(&as[l], &w.opA[set][l][0], 4);
+      memcpy(&bs[l], &w.opB[set][l][0], 4);
+    }
+  }
+  const unsigned col = lane & 15, part = lane >> 4;
+  for(int v = 0; v < 4; v++) {
+    const unsigned row = 4 * part + v;
+    double sum = 0;
+    for(int k = 0; k < 128; k++) {
+      const int p = k % 64 / 16, i = k / 64 * 16 + k % 16, blk = k / 32;
+      sum += (double)decodeE4m3(av[row + 16 * p][i]) * decodeE4m3(bv[col + 16 * p][i]) * ofE8m0(as[row + 16 * blk]) * ofE8m0(bs[col + 16 * blk]);
+    }
+    c[v] += (float)sum;
+  }
+  return c;
+}
+// v_mfma_f32_16x16x32_bf16: lane (row or column l % 16, part l / 16) holds k = 8 part + [0, 8)
+template <class V8, class F4>
+inline F4 mfma16x16(V8 a, V8 b, F4 c) {
+  Wave& w = cur->waves[tIdx.x >> 6];
+  const unsigned lane = tIdx.x & 63, set = waveOp++ & 1;
+  for(int i = 0; i < 8; i++) {
+    w.opA[set][lane][i] = (float)a[i];
+    w.opB[set][lane][i] = (float)b[i];
+  }
+  w.bar->arrive_and_wait();
+  for(int v = 0; v < 4; v++) {
+    float sum = 0.0f;
+    for(int p = 0; p < 4; p++)
+      for(int i = 0; i < 8; i++) sum += w.opA[set][4 * (lane >> 4) + v + 16 * p][i] * w.opB[set][(lane & 15) + 16 * p][i];
+    c[v] += sum;
+  }
+  return c;
+}
 }  // namespace emu
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) emu::cvtPkFp8(a, b, old, hi)
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, hi) emu::cvtBf16Fp8(src, scale, hi)
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) emu::mfmaScale(a, b, c, (int)((unsigned)(sa) >> (8 * (oa))), (int)((unsigned)(sb) >> (8 * (ob))))
+
+#define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) \
+  emu::mfmaScale16(a, b, c, (int)((unsigned)(sa) >> (8 * (oa))), (int)((unsigned)(sb) >> (8 * (ob))))
+#define __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, x, y, z) emu::mfma16x16(a, b, c)
 
 #include "../../katago_amd/csrc/norm_quant.hip"
 #include "../../katago_amd/csrc/linear8.hip"
