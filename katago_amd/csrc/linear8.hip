@@ -31,10 +31,17 @@ typedef const char* Rsrc;
 inline Rsrc bufferOf(const void* p) { return (const char*)p; }
 inline void dma16(Rsrc b, unsigned off, unsigned step, unsigned dst) { emu::globalLoadLds((size_t)b + off + step, (size_t)dst, 16, 0, 0); }
 inline void ldsWrite16(unsigned at, u32x4 v) { *(u32x4*)(size_t)at = v; }
+inline void waveFence() { emu::waveSync(); }
 inline u32x4 ldsRead16(unsigned at) { return *(const u32x4*)(size_t)at; }
 template <int N> inline void waitLoads() { emu::waitVm(N); }
 inline void waitReads0() {}
 inline void waveBarrier() { __syncthreads(); }
+inline int anew(int x) { return x; }
+template <class V> inline void computed(V&) {}
+inline hipError_t computeUnits(int, int* n) {
+  *n = 8;  // (few: work-groups go round more than once)
+  return hipSuccess;
+}
 #else
 __device__ __forceinline__ unsigned ldsAddress(void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) char*)p; }
 // LDS-DMA: the 16 bytes at off (a lane's own) + step (uniform) of a buffer land at dst (uniform) + 16 lane. (As a buffer and not by pointers: no 64-bit
@@ -49,6 +56,9 @@ __device__ __forceinline__ void dma16(Rsrc b, unsigned off, unsigned step, unsig
 }
 __device__ __forceinline__ u32x4 ldsRead16(unsigned at) { return *(const __attribute__((address_space(3))) u32x4*)(size_t)at; }
 __device__ __forceinline__ void ldsWrite16(unsigned at, u32x4 v) { *(__attribute__((address_space(3))) u32x4*)(size_t)at = v; }
+// Lanes of a wave hand data to one another through LDS, whose instructions a wave has carried out in order: only the compiler, which sees one lane's
+// addresses, must not exchange them
+__device__ __forceinline__ void waveFence() { asm volatile("" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void waitLoads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void waitReads0() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -56,6 +66,17 @@ __device__ __forceinline__ void waveBarrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// v is computed by here: products do not move behind the barriers and branches that follow
+template <class V>
+__device__ __forceinline__ void computed(V& v) {
+  asm volatile("" : "+v"(v));
+}
+// x, as far as the compiler can tell a new value each time: what is computed from it is not kept in registers around a loop
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+hipError_t computeUnits(int device, int* n) { return hipDeviceGetAttribute(n, hipDeviceAttributeMultiprocessorCount, device); }
 #endif
 
 template <int I> struct Index { static constexpr int value = I; };
@@ -80,18 +101,22 @@ __device__ __forceinline__ float ofE8m0(unsigned code) {  // 2^(code - 127); 0 i
 typedef unsigned u32u __attribute__((aligned(1)));
 // A row's e8m0 codes of one step, a byte for each 32 k; beyond the row's end 0 (their weights are zeros). The word is fetched in one piece - so that
 // the main loop stays one block, in whose order the products and the barrier stay where they are written - and shifted when it is used.
-__device__ __forceinline__ int codesAt(int blocks, int step) { return step * 4 < blocks - 4 ? step * 4 : blocks - 4; }
+__device__ __forceinline__ int codesAt(int blocks, int step) { return step * 4 < blocks - 4 ? step * 4 : blocks - 4; }  // (below 0: fetched byte by byte)
 __device__ __forceinline__ unsigned fetchCodes(const uint8_t* p, int blocks, int step) { return *(const u32u*)(p + codesAt(blocks, step)); }
-__device__ __forceinline__ unsigned shiftedCodes(unsigned word, int blocks, int step) { return word >> (8 * (step * 4 - codesAt(blocks, step))); }
+__device__ __forceinline__ unsigned shiftedCodes(unsigned word, int blocks, int step) {
+  const int by = 8 * (step * 4 - codesAt(blocks, step));
+  return by < 32 ? word >> by : 0u;
+}
 
-// One BM x BN tile of the output on WM x WN waves. Steps of 128 k: the rows of a and w lie in LDS as they lie in memory, 128 bytes each, the eight
-// pieces of row r at piece ^ ((r >> 1) & 7): the 16 lanes that a ds_read_b128 serves at a time then touch all 64 banks. The pieces are brought
-// by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages. A step multiplies two halves of 64 k: a row tile's fragments
-// are replaced by the next half's as soon as they are used up, the weights' have two sets; the barrier stands behind the second half's first
-// products, when the stage has been read out - it is requested anew there, a whole step ahead of its use. The weights are the matrix instruction's A
-// operand: a lane ends with consecutive output channels of one row of a and stores 16 bytes.
+// BM x BN tiles of the output on WM x WN waves, the work-groups stay and take tile after tile. Steps of 128 k: the rows of a and w lie in LDS as they lie
+// in memory, 128 bytes each, the eight pieces of row r at piece ^ ((r >> 1) & 7): the 16 lanes that a ds_read_b128 serves at a time then touch all 64
+// banks. The pieces are brought by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages. A step multiplies two
+// halves of 64 k: a row tile's fragments are replaced by the next half's as soon as they are used up, the weights' have two sets; the barrier stands
+// behind the second half's first products, when the stage has been read out - it is requested anew there, a whole step ahead of its use. The last two
+// steps of a tile request the first two of the next: a tile's results are scaled and stored while the next one's operands are on their way. The
+// weights are the matrix instruction's A operand: a lane ends with consecutive output channels of one row of a.
 template <int BM, int BN, int WM, int WN, bool MX, int OUT>
-__global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) {
   typedef typename OutTraits<OUT>::TR TR;
   typedef typename TR::T TO;
   constexpr bool EXACT = OUT == DT_F32;
@@ -101,85 +126,118 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   constexpr unsigned STAGE = (unsigned)(BM + BN) * KSTEP;
   HIP_DYNAMIC_SHARED(f32x4, smemLinear8)
   const unsigned lds = ldsAddress(smemLinear8);
-  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + 2 * STAGE);  // [2][BM + BN]: a step's e8m0 codes of each row of a and of w
-  float* const scalesOf = (float*)codesOf;                                  // ... or [BM + BN] the rows' scales; behind either
-  float* const biasOf = (float*)codesOf + 2 * (BM + BN);                    // [BN]
+  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + 2 * STAGE);  // [2][BM + BN]: the e8m0 codes of each row, by step;
+  float* const scalesOf = (float*)codesOf;                                // ... or the rows' scales, by tile
+  float* const biasOf = (float*)codesOf + 2 * (BM + BN);                  // [2][BN], by tile
+  const unsigned patch = lds + 2 * STAGE + (2 * (BM + BN) + 2 * BN) * 4;  // 2 KB of each wave: what is being stored
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hh = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
+  const int pieces = g.K / 16, blocks = MX ? g.K / MX_BLOCK : 0;
+  const int steps = g.K > 2 * KSTEP ? (g.K + KSTEP - 1) / KSTEP : 3;  // at least three: whatever lies beyond K has weights of zero
 
   // Work-groups go round the 8 XCDs one by one: each XCD takes a contiguous eighth of the tiles, in strips of 8 tiles of rows, so that what runs at
   // a time on an XCD shares rows of a and of w in its L2
-  const unsigned mTiles = (unsigned)((g.rows + BM - 1) / BM), nTiles = (unsigned)(g.N + BN - 1) / BN;
-  unsigned tile = blockIdx.x;
-  {
-    const unsigned all = mTiles * nTiles, xcd = tile & 7, each = all >> 3, more = all & 7;
-    tile = xcd * each + (xcd < more ? xcd : more) + (tile >> 3);
-  }
-  const unsigned strip = tile / (8 * nTiles), in = tile % (8 * nTiles), tall = mTiles - strip * 8 < 8 ? mTiles - strip * 8 : 8;
-  const int64_t m0 = (int64_t)(strip * 8 + in % tall) * BM;
-  const int n0 = (int)(in / tall) * BN;
-  const int steps = (g.K + KSTEP - 1) / KSTEP, pieces = g.K / 16;
-  const int mLast = (int)(g.rows - m0 < BM ? g.rows - m0 : BM) - 1, nLast = (g.N - n0 < BN ? g.N - n0 : BN) - 1;  // of this tile
-
-  // rows beyond the matrix are fetched from its last row: their products end in rows / channels that are not stored
-  const uint8_t* const aTile = g.a + m0 * g.aStride;
-  const uint8_t* const wTile = g.w + (int64_t)n0 * g.wStride;
-  unsigned off[REQ_A + REQ_W];
-  auto pieceOf = [&](int r) { return (lane & 7) ^ ((r >> 1) & 7); };
-  auto rowOf = [&](int j) { return (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8 + (lane >> 3); };
-#pragma unroll
-  for(int j = 0; j < REQ_A + REQ_W; j++) {
-    const int r = rowOf(j), last = j < REQ_A ? mLast : nLast;
-    off[j] = (unsigned)(r < last ? r : last) * (unsigned)(j < REQ_A ? g.aStride : g.wStride) + (unsigned)pieceOf(r) * 16;
-  }
-  const Rsrc aRsrc = bufferOf(aTile), wRsrc = bufferOf(wTile);
-  // CUT: the step that holds the end of K. Pieces beyond it are fetched as the row's last one; the weights' are zeroed before they are multiplied
-  auto issue = [&](int step, auto cutTag) {
-    const unsigned stage = lds + (unsigned)(step & 1) * STAGE;
-#pragma unroll
-    for(int j = 0; j < REQ_A + REQ_W; j++) {
-      const unsigned dst = stage + (unsigned)((j < REQ_A ? 0 : BM) + (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8) * KSTEP;
-      unsigned from = off[j];
-      if constexpr(decltype(cutTag)::value != 0) {
-        const int over = step * KPIECES + pieceOf(rowOf(j)) - (pieces - 1);
-        from -= over > 0 ? (unsigned)over * 16 : 0;
-      }
-      dma16(j < REQ_A ? aRsrc : wRsrc, from, (unsigned)step * KSTEP, dst);
-    }
+  const unsigned mTiles = (unsigned)((g.rows + BM - 1) / BM), nTiles = (unsigned)(g.N + BN - 1) / BN, allTiles = mTiles * nTiles;
+  struct Tile {
+    int64_t m0;
+    int n0, mLast, nLast;  // the last row and channel of it that exist
+  };
+  auto tileAt = [&](unsigned id) {
+    const unsigned xcd = id & 7, each = allTiles >> 3, more = allTiles & 7;
+    const unsigned at = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+    const unsigned strip = at / (8 * nTiles), in = at % (8 * nTiles), tall = mTiles - strip * 8 < 8 ? mTiles - strip * 8 : 8;
+    Tile t;
+    t.m0 = (int64_t)(strip * 8 + in % tall) * BM;
+    t.n0 = (int)(in / tall) * BN;
+    t.mLast = (int)(g.rows - t.m0 < BM ? g.rows - t.m0 : BM) - 1;
+    t.nLast = (g.N - t.n0 < BN ? g.N - t.n0 : BN) - 1;
+    return t;
   };
 
-  // e8m0 codes: a thread fetches one row's of a step and puts them into LDS half a step later
-  const int blocks = MX ? g.K / MX_BLOCK : 0;
+  // What is requested: rows beyond the matrix are fetched from its last row (their products end in rows / channels that are not stored), pieces beyond
+  // K as the row's last one (the weights' are zeroed before they are multiplied; a's are finite, or a NaN that the row has anyway).
+  unsigned off[REQ_A + REQ_W];
+  Rsrc aRsrc = bufferOf(g.a), wRsrc = bufferOf(g.w);
+  auto pieceOf = [&](int r, int lane) { return (lane & 7) ^ ((r >> 1) & 7); };
+  auto rowOf = [&](int j, int lane) { return (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8 + (lane >> 3); };
+  auto aim = [&](const Tile& t) {
+    const int ln = anew(lane);
+    aRsrc = bufferOf(g.a + t.m0 * g.aStride);
+    wRsrc = bufferOf(g.w + (int64_t)t.n0 * g.wStride);
+    const unsigned piece = (unsigned)pieceOf(rowOf(0, ln), ln) * 16;  // (rows of one lane differ by multiples of 16: one place of the eight)
+    static_assert(NW % 2 == 0, "pieces");
+    if(t.mLast == BM - 1 && t.nLast == BN - 1) {
+      off[0] = (unsigned)rowOf(0, ln) * (unsigned)g.aStride + piece;
+      off[REQ_A] = (unsigned)rowOf(REQ_A, ln) * (unsigned)g.wStride + piece;
+#pragma unroll
+      for(int j = 1; j < REQ_A; j++) off[j] = off[0] + (unsigned)(j * NW * 8) * (unsigned)g.aStride;
+#pragma unroll
+      for(int j = 1; j < REQ_W; j++) off[REQ_A + j] = off[REQ_A] + (unsigned)(j * NW * 8) * (unsigned)g.wStride;
+    }
+    else {
+#pragma unroll
+      for(int j = 0; j < REQ_A + REQ_W; j++) {
+        const int r = rowOf(j, ln), last = j < REQ_A ? t.mLast : t.nLast;
+        off[j] = (unsigned)(r < last ? r : last) * (unsigned)(j < REQ_A ? g.aStride : g.wStride) + piece;
+      }
+    }
+  };
+  auto issueOne = [&](int j, int step, int parity, auto cutTag, int ln) {  // CUT: pieces of this step may lie beyond K
+    const unsigned dst = lds + (unsigned)parity * STAGE + (unsigned)((j < REQ_A ? 0 : BM) + (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8) * KSTEP;
+    if constexpr(decltype(cutTag)::value != 0) {
+      const int over = step * KPIECES + pieceOf(rowOf(j, ln), ln) - (pieces - 1);
+      dma16(j < REQ_A ? aRsrc : wRsrc, off[j] + (unsigned)step * KSTEP - (over > 0 ? (unsigned)over * 16 : 0), 0, dst);
+    }
+    else dma16(j < REQ_A ? aRsrc : wRsrc, off[j], (unsigned)step * KSTEP, dst);
+  };
+  auto issue = [&](int step, int parity) {
+    const int ln = anew(lane);
+#pragma unroll
+    for(int j = 0; j < REQ_A + REQ_W; j++) issueOne(j, step, parity, Index<1>(), ln);
+  };
+
+  // A thread fetches one row's e8m0 codes of a step and puts them into LDS a step later; or one row's scale of a tile, and the bias
   const int codeRow = (int)threadIdx.x < BM + BN ? (int)threadIdx.x : BM + BN - 1;
   const bool ofA = codeRow < BM;
-  const int64_t scaleRow = ofA ? m0 + (codeRow < mLast ? codeRow : mLast) : n0 + (codeRow - BM < nLast ? codeRow - BM : nLast);
-  const uint8_t* const myCodes = (const uint8_t*)(ofA ? g.aScales : g.wScales) + scaleRow * blocks;
+  auto scaleRow = [&](const Tile& t) {
+    return ofA ? t.m0 + (codeRow < t.mLast ? codeRow : t.mLast) : t.n0 + (codeRow - BM < t.nLast ? codeRow - BM : t.nLast);
+  };
+  const uint8_t* myCodes = nullptr;
   unsigned fetched = 0;
-  auto putCodes = [&](int step) {
-    if constexpr(MX) codesOf[(step & 1) * (BM + BN) + codeRow] = shiftedCodes(fetched, blocks, step);
+  auto putCodes = [&](int step, int parity) {
+    if constexpr(MX) codesOf[parity * (BM + BN) + codeRow] = shiftedCodes(fetched, blocks, step);
+  };
+  auto fetchAny = [&](int step) {
+    if(blocks >= 4) return fetchCodes(myCodes, blocks, step);
+    unsigned v = 0;
+    for(int q = 0; q < blocks; q++) v |= (unsigned)myCodes[q] << (8 * (q + 4 - blocks));  // (as the word that is shifted)
+    return v;
+  };
+  float myScale = 0.0f, myBias = 0.0f;
+  auto fetchScales = [&](const Tile& t) {
+    const int64_t row = scaleRow(t);
+    if constexpr(!MX) myScale = ((const float*)(ofA ? g.aScales : g.wScales))[row];
+    if(g.bias != nullptr) myBias = g.bias[ofA ? 0 : row];
+  };
+  auto putScales = [&](int parity) {
+    if constexpr(!MX) scalesOf[parity * (BM + BN) + codeRow] = myScale;
+    if(!ofA) biasOf[parity * BN + codeRow - BM] = myBias;
   };
 
   f32x16 acc[NI][MI];
-#pragma unroll
-  for(int ni = 0; ni < NI; ni++)
-#pragma unroll
-    for(int mi = 0; mi < MI; mi++)
-#pragma unroll
-      for(int v = 0; v < 16; v++) acc[ni][mi][v] = 0.0f;
-
   const unsigned swz = (unsigned)(col >> 1) & 7u;
   // a step is two halves of 64 k; s = 0, 1: pieces 4 s + hh (k 0..31 of the half) and 4 s + 2 + hh (k 32..63)
   u32x4 fa[MI][2], fw[2][NI][2];
-  auto rowsOf = [&](int step, int base) { return lds + (unsigned)(step & 1) * STAGE + (unsigned)(base + col) * KSTEP; };
+  auto rowsOf = [&](int parity, int base) { return lds + (unsigned)parity * STAGE + (unsigned)(base + col) * KSTEP; };
   auto pieceAt = [&](int p) { return ((unsigned)(p + hh) ^ swz) * 16; };
-  auto readA = [&](int step, int s, int mi) {
-    const unsigned rows = rowsOf(step, wm * TM) + mi * 32 * KSTEP;
+  auto readA = [&](int parity, int s, int mi) {
+    const unsigned rows = rowsOf(parity, wm * TM) + mi * 32 * KSTEP;
     fa[mi][0] = ldsRead16(rows + pieceAt(4 * s));
     fa[mi][1] = ldsRead16(rows + pieceAt(4 * s + 2));
   };
-  auto readW = [&](int step, int s) {
-    const unsigned rows = rowsOf(step, BM + wn * TN);
+  auto readW = [&](int parity, int s) {
+    const unsigned rows = rowsOf(parity, BM + wn * TN);
 #pragma unroll
     for(int ni = 0; ni < NI; ni++) {
       fw[s][ni][0] = ldsRead16(rows + ni * 32 * KSTEP + pieceAt(4 * s));
@@ -189,9 +247,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
   // The instruction takes the scale of k 0..31 from lanes 0..31 and that of k 32..63 from lanes 32..63: its byte 2 s of a step's four, shifted by hh
   // here. (The bf16 way needs both of a half's in every lane.)
   unsigned aCodes[MX ? MI : 1], wCodes[MX ? NI : 1], aNext[MX ? MI : 1], wNext[MX ? NI : 1];
-  auto readCodes = [&](int step) {
+  auto readCodes = [&](int parity) {
     if constexpr(MX) {
-      const unsigned* const c = codesOf + (step & 1) * (BM + BN);
+      const unsigned* const c = codesOf + parity * (BM + BN);
 #pragma unroll
       for(int mi = 0; mi < MI; mi++) aNext[mi] = c[wm * TM + mi * 32 + col] >> (EXACT ? 0 : 8 * hh);
 #pragma unroll
@@ -206,182 +264,253 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8Kernel(Linear8Args g) {
       for(int ni = 0; ni < NI; ni++) wCodes[ni] = wNext[ni];
     }
   };
-  auto multiply = [&](auto sTag, int mi) {
+  auto multiply = [&](auto sTag, int mi, int ni) {
     constexpr int s = decltype(sTag)::value;
     if constexpr(EXACT) {
 #pragma unroll
       for(int q = 0; q < 4; q++) {  // 16 k: 8 codes of each half wave
         const int blk = 2 * s + (q >> 1), e = 2 * (q & 1);
         const Bf8 ba = bf16Of(fa[mi][q >> 1][e], fa[mi][q >> 1][e + 1], MX ? ofE8m0(aCodes[MX ? mi : 0] >> (8 * blk) & 255u) : 1.0f);
-#pragma unroll
-        for(int ni = 0; ni < NI; ni++)
-          acc[ni][mi] = TraitsBF16::mfma(bf16Of(fw[s][ni][q >> 1][e], fw[s][ni][q >> 1][e + 1], MX ? ofE8m0(wCodes[MX ? ni : 0] >> (8 * blk) & 255u) : 1.0f), ba,
-                                         acc[ni][mi]);
+        const Bf8 bw = bf16Of(fw[s][ni][q >> 1][e], fw[s][ni][q >> 1][e + 1], MX ? ofE8m0(wCodes[MX ? ni : 0] >> (8 * blk) & 255u) : 1.0f);
+        acc[ni][mi] = TraitsBF16::mfma(bw, ba, acc[ni][mi]);
       }
     }
     else {
       constexpr int UNIT = 0x7f7f7f7f;
-      i32x8 xa;
+      i32x8 xa, xw;
 #pragma unroll
-      for(int i = 0; i < 8; i++) xa[i] = (int)fa[mi][i >> 2][i & 3];
-#pragma unroll
-      for(int ni = 0; ni < NI; ni++) {
-        i32x8 xw;
-#pragma unroll
-        for(int i = 0; i < 8; i++) xw[i] = (int)fw[s][ni][i >> 2][i & 3];
-        acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw, xa, acc[ni][mi], 0, 0, 2 * s, MX ? (int)wCodes[MX ? ni : 0] : UNIT, 2 * s,
-                                                                      MX ? (int)aCodes[MX ? mi : 0] : UNIT);
+      for(int i = 0; i < 8; i++) {
+        xa[i] = (int)fa[mi][i >> 2][i & 3];
+        xw[i] = (int)fw[s][ni][i >> 2][i & 3];
       }
+      acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw, xa, acc[ni][mi], 0, 0, 2 * s, MX ? (int)wCodes[MX ? ni : 0] : UNIT, 2 * s,
+                                                                    MX ? (int)aCodes[MX ? mi : 0] : UNIT);
     }
   };
+  auto zeroBeyond = [&](int step, int s) {
+#pragma unroll
+    for(int b = 0; b < 2; b++) {
+      const unsigned keep = step * KPIECES + 4 * s + 2 * b + hh < pieces ? 0xffffffffu : 0u;
+#pragma unroll
+      for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+        for(int i = 0; i < 4; i++) fw[s][ni][b][i] &= keep;
+    }
+  };
+  auto pin = [&]() {
+#pragma unroll
+    for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+      for(int mi = 0; mi < MI; mi++) computed(acc[ni][mi]);
+  };
 
-  const int wholeSteps = pieces / KPIECES;  // steps or steps - 1
-  auto issueAny = [&](int step) {
-    if(step < wholeSteps) issue(step, Index<0>());
-    else issue(step, Index<1>());
-  };
-  auto zeroBeyond = [&](int step, int s) {  // (whatever the rows of a hold there: finite, or a NaN that the row has anyway)
-#pragma unroll
-    for(int b = 0; b < 2; b++)
-      if(step * KPIECES + 4 * s + 2 * b + hh >= pieces) {
-#pragma unroll
-        for(int ni = 0; ni < NI; ni++)
-#pragma unroll
-          for(int i = 0; i < 4; i++) fw[s][ni][b][i] = 0;
-      }
-  };
-  constexpr int NOTHING = 0, WHOLE = 1, CUT = 2;  // what a step requests for two steps on
-  auto body = [&](int step, auto moreTag, auto requestTag) {
-    constexpr bool MORE = decltype(moreTag)::value != 0;
-    constexpr int REQUEST = decltype(requestTag)::value;
+  // One step. The stage of this parity is requested anew, with step `want` of the tile that is aimed at; a request holds a wave's issue for as long as
+  // a product takes, so they are spread among the products behind the barrier. Products and barrier stay in this order because there is no branch
+  // between them. youngerTag: how many memory
+  // instructions younger than the next stage's requests may be under way at the barrier.
+  constexpr int INSIDE = 0, END = 1;  // END: one of a tile's last steps - K may end in it, and what it requests
+  auto body = [&](int step, int parity, int want, int wantCodes, auto kindTag, auto youngerTag) {
+    constexpr int KIND = decltype(kindTag)::value;
     takeCodes();
-    readW(step, 1);
-    if constexpr(!MORE)
-      if(wholeSteps < steps) {
+    readW(parity, 1);
+    if constexpr(KIND == END)
+      if((step + 1) * KPIECES > pieces) {
         zeroBeyond(step, 0);
         zeroBeyond(step, 1);
       }
+    unsigned next = 0;
+    if constexpr(MX && KIND == END) next = fetchAny(want);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for(int mi = 0; mi < MI; mi++) {
-      multiply(Index<0>(), mi);
+#pragma unroll
+      for(int ni = 0; ni < NI; ni++) multiply(Index<0>(), mi, ni);
       __builtin_amdgcn_sched_barrier(0);  // (the fragment's registers are free now)
-      readA(step, 1, mi);
+      readA(parity, 1, mi);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr(MORE) putCodes(step + 1);
-    multiply(Index<1>(), 0);
+    putCodes(wantCodes, parity ^ 1);
+#pragma unroll
+    for(int ni = 0; ni < NI; ni++) multiply(Index<1>(), 0, ni);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr(MORE) {
-      waitLoads<0>();   // the next stage is there,
-      waitReads0();   // this one has been read out by this wave,
-      waveBarrier();  // by all of them
-      if constexpr(REQUEST != NOTHING) {
-        if constexpr(MX) fetched = fetchCodes(myCodes, blocks, step + 2);
-        issue(step + 2, Index<REQUEST == CUT ? 1 : 0>());
-      }
-      readCodes(step + 1);
-      readW(step + 1, 0);
-      readA(step + 1, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    if constexpr(KIND == END) pin();
+    waitLoads<decltype(youngerTag)::value>();  // the next stage is there,
+    waitReads0();                              // this one has been read out by this wave,
+    waveBarrier();                             // by all of them
+    if constexpr(MX) fetched = KIND == END ? next : fetchCodes(myCodes, blocks, want);
+    readCodes(parity ^ 1);
+    readW(parity ^ 1, 0);
+    readA(parity ^ 1, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int REQ = REQ_A + REQ_W, SLOTS = MI > 1 ? (MI - 1) * NI : 1;
+    const int ln = KIND == END ? anew(lane) : 0;
+    auto requestsOf = [&](int slot) {
+#pragma unroll
+      for(int j = 0; j < REQ; j++)
+        if(j * SLOTS / REQ == slot) issueOne(j, want, parity, Index<KIND>(), ln);
+    };
+    if constexpr(MI == 1) requestsOf(0);
 #pragma unroll
     for(int mi = 1; mi < MI; mi++) {
-      multiply(Index<1>(), mi);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr(MORE) readA(step + 1, 0, mi);
+#pragma unroll
+      for(int ni = 0; ni < NI; ni++) {
+        requestsOf((mi - 1) * NI + ni);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(Index<1>(), mi, ni);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      readA(parity ^ 1, 0, mi);
       __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr(KIND == END) pin();
   };
 
-  // both stages are requested at once; what the epilogue needs and the codes come in front of them
-  const float myScale = MX ? 0.0f : ((const float*)(ofA ? g.aScales : g.wScales))[scaleRow];
-  const float myBias = ofA || g.bias == nullptr ? 0.0f : g.bias[scaleRow];
+  // Scales, bias, the output's type, and the way to memory: some rows at a time through 2 KB of the wave's own, so that a store instruction covers whole
+  // lines (16 bytes a lane straight from the accumulators' layout: 4 % slower at 92416 x 1152 x 384). Element v of a lane: channel
+  // 8 (v / 4) + 4 hh + v % 4 of the 32, row `col`; piece p of 16 bytes of a row lies at p ^ (row & SWZ). A tile that is whole has no branch here.
+  auto store = [&](const Tile& t, int parity, auto wholeTag) {
+    constexpr bool WHOLE = decltype(wholeTag)::value != 0;
+    constexpr int PER = 16 / (int)sizeof(TO), P = TN / PER, ROWS = 2048 / (P * 16);  // elements of a piece, pieces of a row, rows of a patch
+    constexpr int SWZ = (P < ROWS / 2 ? P : ROWS / 2) - 1 < 7 ? (P < ROWS / 2 ? P : ROWS / 2) - 1 : 7;
+    static_assert(ROWS >= 8 && ROWS <= 32 && (P & (P - 1)) == 0, "patch");
+    static_assert(64 / P == ROWS / 2 && ((ROWS / 2) & SWZ) == 0, "a lane reads and stores a piece of row lane / P, and the same ROWS / 2 rows on");
+    const unsigned mine = patch + (unsigned)wave * 2048;
+    const int ln = anew(lane), col = ln & 31, hh = ln >> 5;
+    const float* const sc = scalesOf + parity * (BM + BN);
+    const float* const bi = biasOf + parity * BN + wn * TN;
+    TO* const corner = (TO*)g.out + (t.m0 + wm * TM) * g.outStride + t.n0 + wn * TN;
+    const int rowsLeft = t.mLast - wm * TM, colsLeft = t.nLast - wn * TN;  // last row / channel of this wave's part
+    const unsigned from = mine + (unsigned)(ln / P * P + (ln % P ^ (ln / P & SWZ))) * 16;
+    const unsigned mineTo = (unsigned)(ln / P) * (unsigned)g.outStride * (unsigned)sizeof(TO) + (unsigned)(ln % P) * 16;
+    auto put = [&](int row0, u32x4 v) {
+      TO* const to = (TO*)((char*)(corner + (int64_t)row0 * g.outStride) + mineTo);
+      if(WHOLE) *(Out16*)to = v;
+      else if(row0 + ln / P <= rowsLeft) {
+        const int c = ln % P * PER;
+        if(c + PER - 1 <= colsLeft) *(Out16*)to = v;
+        else {
+          struct Elements { TO e[PER]; };
+          const Elements e = __builtin_bit_cast(Elements, v);
+#pragma unroll
+          for(int k = 0; k < PER; k++)
+            if(c + k <= colsLeft) to[k] = e.e[k];
+        }
+      }
+    };
+#pragma unroll
+    for(int mi = 0; mi < MI; mi++) {
+      const float sa = MX ? 1.0f : sc[wm * TM + mi * 32 + col];
+      u32x4 out[NI][OUT == DT_F32 ? 4 : 2];  // fp32: pieces of channels 8 q + 4 hh + [0, 4); 16 bits: 16 j + 8 hh + [0, 8)
+#pragma unroll
+      for(int ni = 0; ni < NI; ni++) {
+        u32x2 pk[4];
+#pragma unroll
+        for(int q = 0; q < 4; q++) {
+          const f32x4 bias = *(const f32x4*)(bi + ni * 32 + 8 * q + 4 * hh);
+          f32x4 sw = bias, o;
+          if(!MX) sw = *(const f32x4*)(sc + BM + wn * TN + ni * 32 + 8 * q + 4 * hh);
+#pragma unroll
+          for(int i = 0; i < 4; i++) o[i] = (MX ? acc[ni][mi][4 * q + i] : acc[ni][mi][4 * q + i] * sa * sw[i]) + bias[i];
+          if constexpr(OUT == DT_F32) out[ni][q] = __builtin_bit_cast(u32x4, o);
+          else {
+            typename TR::V4 h;
+#pragma unroll
+            for(int i = 0; i < 4; i++) h[i] = TR::fromFloat(o[i]);
+            pk[q] = __builtin_bit_cast(u32x2, h);
+          }
+        }
+        if constexpr(OUT != DT_F32) {
+          u32x4 two[2];
+          pairUp(pk, two);
+          out[ni][0] = two[0];
+          out[ni][1] = two[1];
+        }
+      }
+#pragma unroll
+      for(int r0 = 0; r0 < 32; r0 += ROWS) {
+        if(ROWS == 32 || (col >= r0 && col < r0 + ROWS)) {
+          const int r = col - r0;
+#pragma unroll
+          for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+            for(int j = 0; j < (OUT == DT_F32 ? 4 : 2); j++) {
+              const int p = ni * (32 / PER) + 2 * j + hh;
+              ldsWrite16(mine + (unsigned)(r * P + (p ^ (r & SWZ))) * 16, out[ni][j]);
+            }
+        }
+        waveFence();  // (a wave's LDS instructions are carried out in order)
+        const u32x4 v0 = ldsRead16(from), v1 = ldsRead16(from + 1024);
+        waveFence();
+        put(mi * 32 + r0, v0);
+        put(mi * 32 + r0 + ROWS / 2, v1);
+      }
+    }
+  };
+  constexpr int STORES = MI * TN * 32 * (int)sizeof(TO) / 1024;  // a wave's store instructions of a whole tile
+  static_assert(STORES <= 63, "vmcnt");
+
+  unsigned id = blockIdx.x;
+  Tile tile = tileAt(id);
+  aim(tile);
+  if constexpr(MX) myCodes = (const uint8_t*)(ofA ? g.aScales : g.wScales) + scaleRow(tile) * blocks;
+  fetchScales(tile);
   unsigned firstCodes = 0;
   if constexpr(MX) {
-    if(blocks >= 4) firstCodes = fetchCodes(myCodes, blocks, 0);
-    else
-      for(int q = 0; q < blocks; q++) firstCodes |= (unsigned)myCodes[q] << (8 * (q + 4 - blocks));  // (as the shifted word)
-    if(steps > 1) fetched = fetchCodes(myCodes, blocks, 1);
+    firstCodes = fetchAny(0);
+    fetched = fetchAny(1);
   }
-  issueAny(0);
-  if(steps > 1) issueAny(1);
-  if constexpr(!MX) scalesOf[codeRow] = myScale;
-  else codesOf[codeRow] = shiftedCodes(firstCodes, blocks, 0);
-  if(!ofA) biasOf[codeRow - BM] = myBias;
-  if(steps > 1) waitLoads<REQ_A + REQ_W>();
-  else waitLoads<0>();
+  issue(0, 0);
+  issue(1, 1);
+  putScales(0);
+  if constexpr(MX) codesOf[codeRow] = shiftedCodes(firstCodes, blocks, 0);
+  waitLoads<0>();
   waitReads0();
   waveBarrier();
   readCodes(0);
   readW(0, 0);
 #pragma unroll
   for(int mi = 0; mi < MI; mi++) readA(0, 0, mi);
-  int step = 0;
-  for(; step + 2 < wholeSteps; step++) body(step, Index<1>(), Index<WHOLE>());
-  if(step + 2 < steps) body(step++, Index<1>(), Index<CUT>());
-  if(step + 1 < steps) body(step++, Index<1>(), Index<NOTHING>());
-  body(step, Index<0>(), Index<NOTHING>());
-
-  // The tile goes through LDS, so that a store instruction covers whole lines of consecutive rows. Element v of a lane: channel 8 (v / 4) + 4 hh + v % 4
-  // of the 32, row `col`; piece p of 16 bytes of row r lies at p ^ (r & 15).
-  constexpr int PER = 16 / (int)sizeof(TO), P = BN / PER;  // elements of a piece, pieces of a row
-  static_assert(BM * P * 16 <= 2 * (int)STAGE && P >= 8 && (P & (P - 1)) == 0, "the tile fits the stages");
-  constexpr int SWZ = P < 16 ? P - 1 : 15;
-  auto place = [&](int r, int p) { return lds + (unsigned)(r * P + (p ^ (r & SWZ))) * 16; };
-  waveBarrier();  // nobody reads the last stage any more
+  int parity = 0, tileParity = 0;
+  for(;;) {
 #pragma unroll
-  for(int ni = 0; ni < NI; ni++) {
-    const int c0 = wn * TN + ni * 32;
-    f32x4 sw[4], bias[4];
+    for(int ni = 0; ni < NI; ni++)
 #pragma unroll
-    for(int q = 0; q < 4; q++) {
-      if(!MX) sw[q] = *(const f32x4*)(scalesOf + BM + c0 + 8 * q + 4 * hh);
-      bias[q] = *(const f32x4*)(biasOf + c0 + 8 * q + 4 * hh);
+      for(int mi = 0; mi < MI; mi++)
+#pragma unroll
+        for(int v = 0; v < 16; v++) acc[ni][mi][v] = 0.0f;
+    // the stores of the tile before may still be under way at the first barrier: what it waits for was requested in front of them
+    body(0, parity, 2, 1, Index<END>(), Index<STORES>());
+    parity ^= 1;
+    int step = 1;
+    for(; step + 3 < steps; step++, parity ^= 1) body(step, parity, step + 2, step + 1, Index<INSIDE>(), Index<0>());
+    pin();
+    if(step + 2 < steps) {
+      body(step, parity, step + 2, step + 1, Index<END>(), Index<0>());
+      parity ^= 1;
+      step++;
     }
-#pragma unroll
-    for(int mi = 0; mi < MI; mi++) {
-      const int r = wm * TM + mi * 32 + col;
-      const float sa = MX ? 1.0f : scalesOf[r];
-      u32x2 pk[4];
-#pragma unroll
-      for(int q = 0; q < 4; q++) {
-        f32x4 o;
-#pragma unroll
-        for(int i = 0; i < 4; i++) o[i] = (MX ? acc[ni][mi][4 * q + i] : acc[ni][mi][4 * q + i] * sa * sw[q][i]) + bias[q][i];
-        if constexpr(OUT == DT_F32) ldsWrite16(place(r, (c0 + 8 * q + 4 * hh) / 4), __builtin_bit_cast(u32x4, o));
-        else {
-          typename TR::V4 t;
-#pragma unroll
-          for(int i = 0; i < 4; i++) t[i] = TR::fromFloat(o[i]);
-          pk[q] = __builtin_bit_cast(u32x2, t);
-        }
-      }
-      if constexpr(OUT != DT_F32) {
-        u32x4 whole[2];
-        pairUp(pk, whole);  // whole[j]: channels 16 j + 8 hh + [0, 8)
-#pragma unroll
-        for(int j = 0; j < 2; j++) ldsWrite16(place(r, (c0 + 16 * j + 8 * hh) / 8), whole[j]);
-      }
-    }
-  }
-  waitReads0();
-  waveBarrier();
-#pragma unroll 4
-  for(int at = (int)threadIdx.x; at < BM * P; at += 64 * NW) {
-    const int r = at / P, c = at % P * PER;
-    if(r > mLast || c > nLast) continue;
-    const u32x4 v = ldsRead16(place(r, at % P));
-    TO* const out = (TO*)g.out + (m0 + r) * g.outStride + n0 + c;
-    if(c + PER - 1 <= nLast) *(Out16*)out = v;
+    // the next tile from here on (this one again where there is none: requested, not used)
+    const bool last = id + gridDim.x >= allTiles;
+    const Tile next = last ? tile : tileAt(id + gridDim.x);
+    aim(next);
+    if constexpr(MX) myCodes = (const uint8_t*)(ofA ? g.aScales : g.wScales) + scaleRow(next) * blocks;
+    fetchScales(next);
+    body(step, parity, 0, step + 1, Index<END>(), Index<0>());
+    parity ^= 1;
+    putScales(tileParity ^ 1);
+    body(step + 1, parity, 1, 0, Index<END>(), Index<0>());
+    parity ^= 1;
+    if(tile.mLast == BM - 1 && tile.nLast == BN - 1) store(tile, tileParity, Index<1>());
     else {
-      struct Elements { TO e[PER]; };
-      const Elements t = __builtin_bit_cast(Elements, v);
-#pragma unroll
-      for(int i = 0; i < PER; i++)
-        if(c + i <= nLast) out[i] = t.e[i];
+      store(tile, tileParity, Index<0>());
+      waitLoads<0>();  // (who knows how many of its lanes had something to store)
     }
+    if(last) break;
+    id += gridDim.x;
+    tile = next;
+    tileParity ^= 1;
   }
+  waitLoads<0>();  // (nothing may land in LDS that is another work-group's by then)
 }
 
 // Few rows: the time is the weights' way from memory, so they go straight into registers, every byte requested at once. A work-group owns 16 output
@@ -515,22 +644,28 @@ template <int BM, int BN, int WM, int WN, bool MX, int OUT>
 hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const int64_t tiles = (g.rows + BM - 1) / BM * ((g.N + BN - 1) / BN);
   if(tiles > 0x7fffffff) return hipErrorInvalidValue;
-  constexpr int LDS = 2 * (BM + BN) * (KSTEP + 4) + BN * 4;
+  constexpr int LDS = 2 * (BM + BN) * KSTEP + (2 * (BM + BN) + 2 * BN) * 4 + WM * WN * 2048, ALL_LDS = 160 * 1024;
+  constexpr int PER_CU = ALL_LDS / LDS < 4 ? ALL_LDS / LDS : 4;  // work-groups of a CU
+  static_assert(PER_CU >= 1, "LDS");
   auto kern = linear8Kernel<BM, BN, WM, WN, MX, OUT>;
-  if(LDS > 64 * 1024) {  // opt in to the large LDS window, once per instantiation and device
-    constexpr int MAX_DEVICES = 64;
-    static std::atomic<bool> attrSet[MAX_DEVICES];
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if(e != hipSuccess) return e;
-    if(dev < 0 || dev >= MAX_DEVICES) return hipErrorInvalidDevice;
-    if(!attrSet[dev].load(std::memory_order_acquire)) {
+  constexpr int MAX_DEVICES = 64;
+  static std::atomic<int> cus[MAX_DEVICES];  // 0: not asked yet
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if(e != hipSuccess) return e;
+  if(dev < 0 || dev >= MAX_DEVICES) return hipErrorInvalidDevice;
+  int n = cus[dev].load(std::memory_order_acquire);
+  if(n == 0) {  // once per instantiation and device
+    if(LDS > 64 * 1024) {  // opt in to the large LDS window
       e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
       if(e != hipSuccess) return e;
-      attrSet[dev].store(true, std::memory_order_release);
     }
+    e = computeUnits(dev, &n);
+    if(e != hipSuccess) return e;
+    cus[dev].store(n, std::memory_order_release);
   }
-  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * WM * WN), LDS, stream, g);
+  const int64_t most = (int64_t)n * PER_CU / 8 * 8;  // (a multiple of the XCDs: a work-group's tiles stay on its XCD's part)
+  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles < most ? tiles : most)), dim3(64 * WM * WN), LDS, stream, g);
   return hipGetLastError();
 }
 template <bool MX, int OUT>
@@ -538,10 +673,17 @@ hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
   if(g.rows <= 16) return launchFew<1, MX, OUT>(g, stream);
   if(g.rows <= 32) return launchFew<2, MX, OUT>(g, stream);
   if(g.rows <= 64) return launchFew<4, MX, OUT>(g, stream);
-  auto tiles = [&](int bm, int bn) { return (g.rows + bm - 1) / bm * ((g.N + bn - 1) / bn); };
+  // A CU holds one work-group of the 256 x 256 tile or two of the 128 x 128: rounds of such sets until all tiles are done, a round of the large
+  // tile measured at 1.6 of a small one's (8192^3: 105 us and 66). The large tile where it needs less time and its edges waste little (92416 rows,
+  // k = 384: n = 1152 in 85 us against 89, but n = 384, half of its second tile empty, in 37 against 28); the small one
+  // while there is a round of it; below that 64 x 64.
+  const int64_t cus = 256;
+  auto tiles = [&](int b) { return (g.rows + b - 1) / b * ((g.N + b - 1) / b); };
+  const int64_t large = tiles(256), small = tiles(128);
   if constexpr(OUT != DT_F32)
-    if(tiles(256, 256) >= 256) return launchTile<256, 256, 2, 4, MX, OUT>(g, stream);
-  if(tiles(128, 128) >= 256) return launchTile<128, 128, 2, 2, MX, OUT>(g, stream);
+    if((large + cus - 1) / cus * 8 < (small + 2 * cus - 1) / (2 * cus) * 5 && large * 4 * 20 < small * 23)
+      return launchTile<256, 256, 2, 4, MX, OUT>(g, stream);
+  if(small >= cus) return launchTile<128, 128, 2, 2, MX, OUT>(g, stream);
   return launchTile<64, 64, 2, 2, MX, OUT>(g, stream);
 }
 template <int OUT>

@@ -172,7 +172,7 @@ int kmx_linear8(int device, void* stream, const kmx_linear8_args* p) {
     const int dtype = dtypeOf(me, p->out_type);
     const int64_t es = dtSize(dtype), M = p->rows, N = p->n, K = p->k;
     if(M < 0 || M > 0x7fffffff) refuse(me, "rows must be 0 .. 2^31 - 1");
-    if(N < 1 || N > (1 << 28)) refuse(me, "n must be 1 .. 2^28");
+    if(N < 1 || N >= (1 << 23)) refuse(me, "n must be 1 .. 2^23 - 1");
     if(p->scale_kind != SCALES_ROW && p->scale_kind != SCALES_MX) refuse(me, "the scales are KMX_SCALES_ROW or KMX_SCALES_MX");
     const int step = p->scale_kind == SCALES_MX ? MX_BLOCK : 16;
     if(K < step || K % step != 0 || K >= (1 << 23)) refuse(me, "k must be a multiple of " + std::to_string(step) + " below 2^23");
@@ -187,6 +187,7 @@ int kmx_linear8(int device, void* stream, const kmx_linear8_args* p) {
     aligned(me, "out", p->out, (size_t)es);
     if(p->a_stride < 0 || p->w_stride < 0 || p->a_stride % 16 != 0 || p->w_stride % 16 != 0 || p->a_stride >= (1 << 23) || p->w_stride >= (1 << 23))
       refuse(me, "the strides of a and w must be multiples of 16 below 2^23");
+    if(p->out_stride >= (1 << 23)) refuse(me, "out_stride must be below 2^23");
     const Rows out{(const char*)p->out, M, elements(me, "out", M, p->out_stride, N, true) * es, N * es};
     const int64_t perA = p->scale_kind == SCALES_ROW ? 4 : K / MX_BLOCK;
     const Rows in[] = {{(const char*)p->a, M, p->a_stride, K}, {(const char*)p->w, N, p->w_stride, K}, {(const char*)p->a_scales, 1, M * perA, M * perA},

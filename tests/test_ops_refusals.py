@@ -111,7 +111,7 @@ def linear_args(**kw):
     (dict(scale_kind=2, k=48), "32"), (dict(k=1 << 23), "k must"), (dict(scale_kind=0), "scales"), (dict(a=None), "needed"), (dict(w=None), "needed"),
     (dict(a_scales=None), "needed"), (dict(w_scales=None), "needed"), (dict(out=None), "needed"), (dict(a=MB + 8), "aligned"), (dict(w=3 * MB + 1), "aligned"),
     (dict(a_scales=2 * MB + 1), "aligned"), (dict(bias=6 * MB + 2), "aligned"), (dict(out=5 * MB + 1), "aligned"), (dict(a_stride=72), "strides"),
-    (dict(w_stride=-64), "strides"), (dict(a_stride=1 << 23), "strides"), (dict(out_stride=32), "out:"), (dict(out=MB), "overlap"), (dict(out=4 * MB), "overlap"),
+    (dict(w_stride=-64), "strides"), (dict(a_stride=1 << 23), "strides"), (dict(out_stride=32), "out:"), (dict(out_stride=1 << 23), "out_stride"), (dict(n=1 << 23, out_stride=1 << 23), "n must"), (dict(out=MB), "overlap"), (dict(out=4 * MB), "overlap"),
     (dict(bias=5 * MB), "overlap")])
 def test_linear8_refuses(lib, kw, word):
     refused(lib, lib.kmx_linear8(9999, None, ctypes.byref(linear_args(**kw))), "kmx_linear8", word)
