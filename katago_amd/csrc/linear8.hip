@@ -110,12 +110,12 @@ __device__ __forceinline__ unsigned shiftedCodes(unsigned word, int blocks, int 
 
 // BM x BN tiles of the output on WM x WN waves, the work-groups stay and take tile after tile. Steps of 128 k: the rows of a and w lie in LDS as they lie
 // in memory, 128 bytes each, the eight pieces of row r at piece ^ ((r >> 1) & 7): the 16 lanes that a ds_read_b128 serves at a time then touch all 64
-// banks. The pieces are brought by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages. A step multiplies two
+// banks. The pieces are brought by LDS-DMA in that order (the lanes of a request take their pieces' addresses), two stages (or four). A step multiplies two
 // halves of 64 k: a row tile's fragments are replaced by the next half's as soon as they are used up, the weights' have two sets; the barrier stands
 // behind the second half's first products, when the stage has been read out - it is requested anew there, a whole step ahead of its use. The last two
 // steps of a tile request the first two of the next: a tile's results are scaled and stored while the next one's operands are on their way. The
 // weights are the matrix instruction's A operand: a lane ends with consecutive output channels of one row of a.
-template <int BM, int BN, int WM, int WN, bool MX, int OUT>
+template <int BM, int BN, int WM, int WN, int STAGES, bool MX, int OUT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) {
   typedef typename OutTraits<OUT>::TR TR;
   typedef typename TR::T TO;
@@ -126,15 +126,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
   constexpr unsigned STAGE = (unsigned)(BM + BN) * KSTEP;
   HIP_DYNAMIC_SHARED(f32x4, smemLinear8)
   const unsigned lds = ldsAddress(smemLinear8);
-  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + 2 * STAGE);  // [2][BM + BN]: the e8m0 codes of each row, by step;
+  static_assert(STAGES == 2 || STAGES == 4, "ring");
+  unsigned* const codesOf = (unsigned*)((char*)smemLinear8 + STAGES * STAGE);  // [2][BM + BN]: the e8m0 codes of each row, by step;
   float* const scalesOf = (float*)codesOf;                                // ... or the rows' scales, by tile
   float* const biasOf = (float*)codesOf + 2 * (BM + BN);                  // [2][BN], by tile
-  const unsigned patch = lds + 2 * STAGE + (2 * (BM + BN) + 2 * BN) * 4;  // 2 KB of each wave: what is being stored
+  const unsigned patch = lds + STAGES * STAGE + (2 * (BM + BN) + 2 * BN) * 4;  // 2 KB of each wave: what is being stored
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hh = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   const int pieces = g.K / 16, blocks = MX ? g.K / MX_BLOCK : 0;
-  const int steps = g.K > 2 * KSTEP ? (g.K + KSTEP - 1) / KSTEP : 3;  // at least three: whatever lies beyond K has weights of zero
+  // at least one more than there are stages: whatever lies beyond K has weights of zero
+  const int steps = g.K > STAGES * KSTEP ? (g.K + KSTEP - 1) / KSTEP : STAGES + 1;
 
   // Work-groups go round the 8 XCDs one by one: each XCD takes a contiguous eighth of the tiles, in strips of 8 tiles of rows, so that what runs at
   // a time on an XCD shares rows of a and of w in its L2
@@ -183,18 +185,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
       }
     }
   };
-  auto issueOne = [&](int j, int step, int parity, auto cutTag, int ln) {  // CUT: pieces of this step may lie beyond K
-    const unsigned dst = lds + (unsigned)parity * STAGE + (unsigned)((j < REQ_A ? 0 : BM) + (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8) * KSTEP;
+  auto issueOne = [&](int j, int step, int stage, auto cutTag, int ln) {  // CUT: pieces of this step may lie beyond K
+    const unsigned dst = lds + (unsigned)stage * STAGE + (unsigned)((j < REQ_A ? 0 : BM) + (wave + NW * (j < REQ_A ? j : j - REQ_A)) * 8) * KSTEP;
     if constexpr(decltype(cutTag)::value != 0) {
       const int over = step * KPIECES + pieceOf(rowOf(j, ln), ln) - (pieces - 1);
       dma16(j < REQ_A ? aRsrc : wRsrc, off[j] + (unsigned)step * KSTEP - (over > 0 ? (unsigned)over * 16 : 0), 0, dst);
     }
     else dma16(j < REQ_A ? aRsrc : wRsrc, off[j], (unsigned)step * KSTEP, dst);
   };
-  auto issue = [&](int step, int parity) {
+  auto issue = [&](int step, int stage) {
     const int ln = anew(lane);
 #pragma unroll
-    for(int j = 0; j < REQ_A + REQ_W; j++) issueOne(j, step, parity, Index<1>(), ln);
+    for(int j = 0; j < REQ_A + REQ_W; j++) issueOne(j, step, stage, Index<1>(), ln);
   };
 
   // A thread fetches one row's e8m0 codes of a step and puts them into LDS a step later; or one row's scale of a tile, and the bias
@@ -229,15 +231,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
   const unsigned swz = (unsigned)(col >> 1) & 7u;
   // a step is two halves of 64 k; s = 0, 1: pieces 4 s + hh (k 0..31 of the half) and 4 s + 2 + hh (k 32..63)
   u32x4 fa[MI][2], fw[2][NI][2];
-  auto rowsOf = [&](int parity, int base) { return lds + (unsigned)parity * STAGE + (unsigned)(base + col) * KSTEP; };
+  auto rowsOf = [&](int stage, int base) { return lds + (unsigned)stage * STAGE + (unsigned)(base + col) * KSTEP; };
   auto pieceAt = [&](int p) { return ((unsigned)(p + hh) ^ swz) * 16; };
-  auto readA = [&](int parity, int s, int mi) {
-    const unsigned rows = rowsOf(parity, wm * TM) + mi * 32 * KSTEP;
+  auto readA = [&](int stage, int s, int mi) {
+    const unsigned rows = rowsOf(stage, wm * TM) + mi * 32 * KSTEP;
     fa[mi][0] = ldsRead16(rows + pieceAt(4 * s));
     fa[mi][1] = ldsRead16(rows + pieceAt(4 * s + 2));
   };
-  auto readW = [&](int parity, int s) {
-    const unsigned rows = rowsOf(parity, BM + wn * TN);
+  auto readW = [&](int stage, int s) {
+    const unsigned rows = rowsOf(stage, BM + wn * TN);
 #pragma unroll
     for(int ni = 0; ni < NI; ni++) {
       fw[s][ni][0] = ldsRead16(rows + ni * 32 * KSTEP + pieceAt(4 * s));
@@ -304,50 +306,53 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
       for(int mi = 0; mi < MI; mi++) computed(acc[ni][mi]);
   };
 
-  // One step. The stage of this parity is requested anew, with step `want` of the tile that is aimed at; a request holds a wave's issue for as long as
+  // One step: the at-th of this work-group (its stage and codes by that), `step` of its tile. The stage is requested anew, with step `want` of the tile that
+  // is aimed at; a request holds a wave's issue for as long as
   // a product takes, so they are spread among the products behind the barrier. Products and barrier stay in this order because there is no branch
   // between them. youngerTag: how many memory
   // instructions younger than the next stage's requests may be under way at the barrier.
   constexpr int INSIDE = 0, END = 1;  // END: one of a tile's last steps - K may end in it, and what it requests
-  auto body = [&](int step, int parity, int want, int wantCodes, auto kindTag, auto youngerTag) {
+  constexpr int AHEAD = (STAGES - 2) * (REQ_A + REQ_W);  // requests of the stages behind the next
+  auto body = [&](int at, int step, int want, int codesPut, int codesFetch, auto kindTag, auto youngerTag) {
     constexpr int KIND = decltype(kindTag)::value;
+    const int stage = at & (STAGES - 1), after = (at + 1) & (STAGES - 1);
     takeCodes();
-    readW(parity, 1);
+    readW(stage, 1);
     if constexpr(KIND == END)
       if((step + 1) * KPIECES > pieces) {
         zeroBeyond(step, 0);
         zeroBeyond(step, 1);
       }
     unsigned next = 0;
-    if constexpr(MX && KIND == END) next = fetchAny(want);
+    if constexpr(MX && KIND == END) next = fetchAny(codesFetch);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for(int mi = 0; mi < MI; mi++) {
 #pragma unroll
       for(int ni = 0; ni < NI; ni++) multiply(Index<0>(), mi, ni);
       __builtin_amdgcn_sched_barrier(0);  // (the fragment's registers are free now)
-      readA(parity, 1, mi);
+      readA(stage, 1, mi);
       __builtin_amdgcn_sched_barrier(0);
     }
-    putCodes(wantCodes, parity ^ 1);
+    putCodes(codesPut, (at + 1) & 1);
 #pragma unroll
     for(int ni = 0; ni < NI; ni++) multiply(Index<1>(), 0, ni);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr(KIND == END) pin();
-    waitLoads<decltype(youngerTag)::value>();  // the next stage is there,
-    waitReads0();                              // this one has been read out by this wave,
-    waveBarrier();                             // by all of them
-    if constexpr(MX) fetched = KIND == END ? next : fetchCodes(myCodes, blocks, want);
-    readCodes(parity ^ 1);
-    readW(parity ^ 1, 0);
-    readA(parity ^ 1, 0, 0);
+    waitLoads<AHEAD + decltype(youngerTag)::value>();  // the next stage is there,
+    waitReads0();                                      // this one has been read out by this wave,
+    waveBarrier();                                     // by all of them
+    if constexpr(MX) fetched = KIND == END ? next : fetchCodes(myCodes, blocks, codesFetch);
+    readCodes((at + 1) & 1);
+    readW(after, 0);
+    readA(after, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
     constexpr int REQ = REQ_A + REQ_W, SLOTS = MI > 1 ? (MI - 1) * NI : 1;
     const int ln = KIND == END ? anew(lane) : 0;
     auto requestsOf = [&](int slot) {
 #pragma unroll
       for(int j = 0; j < REQ; j++)
-        if(j * SLOTS / REQ == slot) issueOne(j, want, parity, Index<KIND>(), ln);
+        if(j * SLOTS / REQ == slot) issueOne(j, want, stage, Index<KIND>(), ln);
     };
     if constexpr(MI == 1) requestsOf(0);
 #pragma unroll
@@ -359,7 +364,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
         multiply(Index<1>(), mi, ni);
         __builtin_amdgcn_sched_barrier(0);
       }
-      readA(parity ^ 1, 0, mi);
+      readA(after, 0, mi);
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr(KIND == END) pin();
@@ -459,18 +464,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     firstCodes = fetchAny(0);
     fetched = fetchAny(1);
   }
-  issue(0, 0);
-  issue(1, 1);
+#pragma unroll
+  for(int k = 0; k < STAGES; k++) issue(k, k);
   putScales(0);
   if constexpr(MX) codesOf[codeRow] = shiftedCodes(firstCodes, blocks, 0);
-  waitLoads<0>();
+  waitLoads<AHEAD>();
   waitReads0();
   waveBarrier();
   readCodes(0);
   readW(0, 0);
 #pragma unroll
   for(int mi = 0; mi < MI; mi++) readA(0, 0, mi);
-  int parity = 0, tileParity = 0;
+  int at = 0, tileParity = 0;
   for(;;) {
 #pragma unroll
     for(int ni = 0; ni < NI; ni++)
@@ -479,27 +484,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
 #pragma unroll
         for(int v = 0; v < 16; v++) acc[ni][mi][v] = 0.0f;
     // the stores of the tile before may still be under way at the first barrier: what it waits for was requested in front of them
-    body(0, parity, 2, 1, Index<END>(), Index<STORES>());
-    parity ^= 1;
+    body(at++, 0, STAGES, 1, 2, Index<END>(), Index<STORES>());
     int step = 1;
-    for(; step + 3 < steps; step++, parity ^= 1) body(step, parity, step + 2, step + 1, Index<INSIDE>(), Index<0>());
+    for(; step + STAGES + 1 < steps; step++) body(at++, step, step + STAGES, step + 1, step + 2, Index<INSIDE>(), Index<0>());
     pin();
-    if(step + 2 < steps) {
-      body(step, parity, step + 2, step + 1, Index<END>(), Index<0>());
-      parity ^= 1;
+    if(step + STAGES < steps) {
+      body(at++, step, step + STAGES, step + 1, step + 2, Index<END>(), Index<0>());
       step++;
     }
-    // the next tile from here on (this one again where there is none: requested, not used)
+    // the next tile is requested from here on (this one again where there is none: requested, not used)
     const bool last = id + gridDim.x >= allTiles;
     const Tile next = last ? tile : tileAt(id + gridDim.x);
     aim(next);
+    if constexpr(STAGES > 2)
+#pragma unroll 1
+      for(int want = 0; want < STAGES - 2; want++, step++) body(at++, step, want, step + 1, step + 2, Index<END>(), Index<0>());
     if constexpr(MX) myCodes = (const uint8_t*)(ofA ? g.aScales : g.wScales) + scaleRow(next) * blocks;
     fetchScales(next);
-    body(step, parity, 0, step + 1, Index<END>(), Index<0>());
-    parity ^= 1;
+    body(at++, step, STAGES - 2, step + 1, 0, Index<END>(), Index<0>());
     putScales(tileParity ^ 1);
-    body(step + 1, parity, 1, 0, Index<END>(), Index<0>());
-    parity ^= 1;
+    body(at++, step + 1, STAGES - 1, 0, 1, Index<END>(), Index<0>());
     if(tile.mLast == BM - 1 && tile.nLast == BN - 1) store(tile, tileParity, Index<1>());
     else {
       store(tile, tileParity, Index<0>());
@@ -640,14 +644,14 @@ hipError_t launchFew(const Linear8Args& g, hipStream_t stream) {
   hipLaunchKernelGGL(kern, dim3((unsigned)((g.N + 15) / 16), (unsigned)((g.rows + 16 * MT - 1) / (16 * MT))), dim3(512), 0, stream, g);
   return hipGetLastError();
 }
-template <int BM, int BN, int WM, int WN, bool MX, int OUT>
+template <int BM, int BN, int WM, int WN, int STAGES, bool MX, int OUT>
 hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const int64_t tiles = (g.rows + BM - 1) / BM * ((g.N + BN - 1) / BN);
   if(tiles > 0x7fffffff) return hipErrorInvalidValue;
-  constexpr int LDS = 2 * (BM + BN) * KSTEP + (2 * (BM + BN) + 2 * BN) * 4 + WM * WN * 2048, ALL_LDS = 160 * 1024;
+  constexpr int LDS = STAGES * (BM + BN) * KSTEP + (2 * (BM + BN) + 2 * BN) * 4 + WM * WN * 2048, ALL_LDS = 160 * 1024;
   constexpr int PER_CU = ALL_LDS / LDS < 4 ? ALL_LDS / LDS : 4;  // work-groups of a CU
   static_assert(PER_CU >= 1, "LDS");
-  auto kern = linear8Kernel<BM, BN, WM, WN, MX, OUT>;
+  auto kern = linear8Kernel<BM, BN, WM, WN, STAGES, MX, OUT>;
   constexpr int MAX_DEVICES = 64;
   static std::atomic<int> cus[MAX_DEVICES];  // 0: not asked yet
   int dev = 0;
@@ -670,21 +674,27 @@ hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
 }
 template <bool MX, int OUT>
 hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
+  // Few rows: up to 32 on the kernel without LDS (32 x 4096 x 4096 8.1 us; 64 rows 11.7 against 10.0 on 64 x 64 tiles with four stages), up to 64 where k
+  // is too short for those to get going (64 x 1152 x 384 3.0 us against 3.8).
+  const bool longK = g.K >= 8 * KSTEP;
   if(g.rows <= 16) return launchFew<1, MX, OUT>(g, stream);
   if(g.rows <= 32) return launchFew<2, MX, OUT>(g, stream);
-  if(g.rows <= 64) return launchFew<4, MX, OUT>(g, stream);
+  if(g.rows <= 64 && !longK) return launchFew<4, MX, OUT>(g, stream);
   // A CU holds one work-group of the 256 x 256 tile or two of the 128 x 128: rounds of such sets until all tiles are done, a round of the large
   // tile measured at 1.6 of a small one's (8192^3: 105 us and 66). The large tile where it needs less time and its edges waste little (92416 rows,
-  // k = 384: n = 1152 in 85 us against 89, but n = 384, half of its second tile empty, in 37 against 28); the small one
-  // while there is a round of it; below that 64 x 64.
+  // k = 384: n = 1152 in 84 us against 89, but n = 384, half of its second tile empty, in 34 against 28); the small one while there is a
+  // round of it - with one work-group to a CU four stages, which hide a request's time better (1000 x 4096 x 4096 27.1 -> 24.0 us);
+  // below that 64 x 64, with four stages where k is long (128 x 4096 x 4096 16.8 -> 10.0 us, 361 x 1152 x 384 3.8 -> 4.9).
   const int64_t cus = 256;
   auto tiles = [&](int b) { return (g.rows + b - 1) / b * ((g.N + b - 1) / b); };
   const int64_t large = tiles(256), small = tiles(128);
   if constexpr(OUT != DT_F32)
     if((large + cus - 1) / cus * 8 < (small + 2 * cus - 1) / (2 * cus) * 5 && large * 4 * 20 < small * 23)
-      return launchTile<256, 256, 2, 4, MX, OUT>(g, stream);
-  if(small >= cus) return launchTile<128, 128, 2, 2, MX, OUT>(g, stream);
-  return launchTile<64, 64, 2, 2, MX, OUT>(g, stream);
+      return launchTile<256, 256, 2, 4, 2, MX, OUT>(g, stream);
+  if(small > cus) return launchTile<128, 128, 2, 2, 2, MX, OUT>(g, stream);
+  if(!longK) return launchTile<64, 64, 2, 2, 2, MX, OUT>(g, stream);
+  if(small * 8 > cus * 5) return launchTile<128, 128, 2, 2, 4, MX, OUT>(g, stream);
+  return launchTile<64, 64, 2, 2, 4, MX, OUT>(g, stream);
 }
 template <int OUT>
 hipError_t launchScales(const Linear8Args& g, hipStream_t stream) {

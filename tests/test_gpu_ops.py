@@ -161,7 +161,8 @@ def eight(rows, k, scales, g, spread=1.0):
 @pytest.mark.parametrize("out", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("scales", ["row", "mx"])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 4096, 4096), (2, 100, 96), (16, 1000, 512), (17, 64, 2048), (33, 33, 64), (361, 1152, 384), (64, 65, 128),
-                                   (127, 129, 160), (130, 8, 1024), (500, 2000, 256), (2049, 2050, 288), (9000, 200, 96)])
+                                   (127, 129, 160), (130, 8, 1024), (500, 2000, 256), (2049, 2050, 288), (9000, 200, 96),
+                                   (64, 100, 1024), (65, 70, 1040 - 16), (200, 3000, 1184), (1000, 4100, 1152), (1100, 5000, 1056), (5000, 4999, 512), (4100, 16400, 128)])
 def test_linear8(m, n, k, scales, out):
     g = gen(m + n)
     (a, sa), (w, sw) = eight(m, k, scales, g, 2.0), eight(n, k, scales, g, 0.1)
