@@ -117,7 +117,7 @@ def rotary(x, positions, freqs, half_layout, magnitude=1.0, inverse=False):
 
 
 def check_rotary(got, want, size, turn, magnitude=1.0):
-    """The turn's fraction is rounded to fp32 once (2^-25 of a turn: pi U), sine and cosine are good to 2 U, times the magnitude, three roundings of the
+    """The turn's fraction is rounded to fp32 once (2^-25 of a turn: pi U), sine and cosine are good to 2.1 U, times the magnitude, three roundings of the
     rotation: below 10 U of the pair; the angle in fp64 is off by at most 2^-51 of itself (here and in the formula)."""
     t = got.dtype
     far = (got.double() - want).abs()
