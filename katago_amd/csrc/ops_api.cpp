@@ -73,6 +73,37 @@ bool meet(const Rows& a, const Rows& b) {
 }
 bool same(const Rows& a, const Rows& b) { return a.p == b.p && (a.stride == b.stride || a.rows <= 1); }
 
+// A strided tensor of batch x seq x heads rows of head_dim elements, in bytes
+struct Box {
+  const char* p;
+  int64_t len[3], stride[3], width;
+  int64_t span() const { return (len[0] - 1) * stride[0] + (len[1] - 1) * stride[1] + (len[2] - 1) * stride[2] + width; }
+};
+bool tooFar(int64_t stride, int64_t len) { return stride >= (int64_t)1 << 40 || (len > 1 && stride > ((int64_t)1 << 57) / len); }
+// What a box covers of every period of `period` bytes, 0 where it has no such period
+int64_t within(const Box& b, int64_t period) {
+  int64_t w = b.width;
+  for(int d = 0; d < 3; d++) {
+    if(b.len[d] <= 1 || b.stride[d] % period == 0) continue;
+    if(b.stride[d] > period) return 0;
+    w += (b.len[d] - 1) * b.stride[d];
+  }
+  return w;
+}
+// Do two tensors share bytes? Apart are those whose spans are, and columns of one buffer: q and k of a fused projection's output, side by side in a
+// token, in a sequence or in a head. (Stranger interleavings count as shared.)
+bool meet(const Box& a, const Box& b) {
+  if(a.p + a.span() <= b.p || b.p + b.span() <= a.p) return false;
+  for(const Box* of : {&a, &b})
+    for(int d = 0; d < 3; d++) {
+      const int64_t period = of->stride[d];
+      if(of->len[d] <= 1 || period <= 0) continue;
+      const int64_t wa = within(a, period), wb = within(b, period), at = ((b.p - a.p) % period + period) % period;
+      if(wa > 0 && wb > 0 && at >= wa && at + wb <= period) return false;
+    }
+  return true;
+}
+
 int64_t elements(const char* entry, const char* name, int64_t rows, int64_t stride, int64_t width, bool output) {
   if(stride < 0 || (output && rows > 1 && stride < width)) refuse(entry, std::string(name) + ": rows overlap (stride " + std::to_string(stride) + ")");
   if(rows > 0 && stride > ((int64_t)1 << 58) / rows) refuse(entry, std::string(name) + ": the stride is out of range");
@@ -211,6 +242,7 @@ int kmx_rotary(int device, void* stream, const kmx_rotary_args* p) {
     if(p->batch < 0 || p->seq < 0 || (p->seq > 0 && p->batch > 0x7fffffff / p->seq)) refuse(me, "batch * seq must be below 2^31");
     if(p->q_heads < 1 || p->k_heads < 0 || p->q_heads > (1 << 16) || p->k_heads > (1 << 16)) refuse(me, "q_heads must be 1 .. 65536, k_heads 0 .. 65536");
     if(p->head_dim < 2 || p->head_dim > (1 << 16) || p->pairs < 1 || 2 * p->pairs > p->head_dim) refuse(me, "2 <= 2 * pairs <= head_dim <= 65536");
+    if(((int64_t)p->q_heads + p->k_heads) * p->head_dim > 0x7fffffff) refuse(me, "a token's heads must have fewer than 2^31 channels");
     if(p->axes != 1 && p->axes != 2) refuse(me, "axes must be 1 or 2");
     if(p->freq_heads < 1 || p->q_heads % p->freq_heads != 0 || p->k_heads % p->freq_heads != 0) refuse(me, "freq_heads must divide q_heads and k_heads");
     if(p->frequencies == nullptr || p->positions == nullptr) refuse(me, "frequencies and positions are needed");
@@ -219,8 +251,7 @@ int kmx_rotary(int device, void* stream, const kmx_rotary_args* p) {
     if(p->pos_batch_stride < 0 || p->pos_seq_stride < 0 || p->pos_axis_stride < 0) refuse(me, "negative strides");
     if(!(p->magnitude >= -3.0e38f && p->magnitude <= 3.0e38f)) refuse(me, "the magnitude must be finite");
     RotaryArgs a = {};
-    struct Span { const char *lo, *hi; };
-    Span in[2] = {}, out[2] = {};
+    Box in[2], out[2];
     const kmx_rotary_tensor* const t[2] = {&p->q, &p->k};
     const int heads[2] = {p->q_heads, p->k_heads};
     const bool any = p->batch > 0 && p->seq > 0;
@@ -234,14 +265,9 @@ int kmx_rotary(int device, void* stream, const kmx_rotary_args* p) {
       aligned(me, name.c_str(), x.out, (size_t)es);
       const int64_t si[3] = {x.in_batch_stride, x.in_seq_stride, x.in_head_stride}, so[3] = {x.out_batch_stride, x.out_seq_stride, x.out_head_stride};
       const int64_t len[3] = {p->batch, p->seq, heads[i]};
-      int64_t spanIn = p->head_dim, spanOut = p->head_dim;
       for(int d = 0; d < 3; d++) {
         if(si[d] < 0 || so[d] < 0) refuse(me, name + ": negative strides");
-        if(si[d] >= ((int64_t)1 << 40) || so[d] >= ((int64_t)1 << 40)) refuse(me, name + ": a stride is out of range");
-        if(any) {
-          spanIn += (len[d] - 1) * si[d];
-          spanOut += (len[d] - 1) * so[d];
-        }
+        if(tooFar(si[d], len[d]) || tooFar(so[d], len[d])) refuse(me, name + ": a stride is out of range");
       }
       // an output's elements are apart: sorted by stride, each dimension steps over all that the smaller ones span
       int order[3] = {0, 1, 2};
@@ -254,33 +280,24 @@ int kmx_rotary(int device, void* stream, const kmx_rotary_args* p) {
         if(so[d] < inner) refuse(me, name + ": the output's elements overlap");
         inner += (len[d] - 1) * so[d];
       }
-      in[i] = Span{(const char*)x.in, (const char*)x.in + spanIn * es};
-      out[i] = Span{(const char*)x.out, (const char*)x.out + spanOut * es};
+      in[i] = Box{(const char*)x.in, {len[0], len[1], len[2]}, {si[0] * es, si[1] * es, si[2] * es}, p->head_dim * es};
+      out[i] = Box{(const char*)x.out, {len[0], len[1], len[2]}, {so[0] * es, so[1] * es, so[2] * es}, p->head_dim * es};
       const bool inPlace = x.in == x.out && (len[0] <= 1 || si[0] == so[0]) && (len[1] <= 1 || si[1] == so[1]) && (len[2] <= 1 || si[2] == so[2]);
-      if(!inPlace && any && in[i].lo < out[i].hi && out[i].lo < in[i].hi) refuse(me, name + ": out overlaps in and is not in itself");
+      if(!inPlace && any && meet(in[i], out[i])) refuse(me, name + ": out overlaps in and is not in itself");
       RotarySide& s = a.side[i];
       s.in = x.in; s.out = x.out;
       s.inBatch = si[0]; s.inToken = si[1]; s.inHead = si[2]; s.outBatch = so[0]; s.outToken = so[1]; s.outHead = so[2];
     }
-    // q and k may be columns of one buffer (a fused projection's output): their spans then cross, but not their rows
-    auto apart = [&](const char* u, int64_t uBatch, int64_t uSeq, int64_t uHead, int uHeads, const char* v, int64_t vBatch, int64_t vSeq, int64_t vHead, int vHeads) {
-      const int64_t row = p->seq > 1 ? uSeq : uBatch;
-      if(row <= 0 || row != (p->seq > 1 ? vSeq : vBatch)) return false;
-      if(p->seq > 1 && p->batch > 1 && (uBatch % row != 0 || vBatch % row != 0)) return false;
-      const int64_t r = row * es, uWidth = ((uHeads - 1) * uHead + p->head_dim) * es, vWidth = ((vHeads - 1) * vHead + p->head_dim) * es;
-      const int64_t d = ((v - u) % r + r) % r;
-      return d >= uWidth && d + vWidth <= r;
-    };
-    auto cross = [](const Span& u, const Span& v) { return u.lo < v.hi && v.lo < u.hi; };
-    if(heads[1] > 0 && any && p->batch * p->seq > 1) {
-      const RotarySide &q = a.side[0], &k = a.side[1];
-      const char *qo = (const char*)q.out, *ko = (const char*)k.out;
-      if((cross(out[0], out[1]) && !apart(qo, q.outBatch, q.outToken, q.outHead, q.heads, ko, k.outBatch, k.outToken, k.outHead, k.heads)) ||
-         (cross(out[0], in[1]) && !apart(qo, q.outBatch, q.outToken, q.outHead, q.heads, (const char*)k.in, k.inBatch, k.inToken, k.inHead, k.heads)) ||
-         (cross(in[0], out[1]) && !apart((const char*)q.in, q.inBatch, q.inToken, q.inHead, q.heads, ko, k.outBatch, k.outToken, k.outHead, k.heads)))
-        refuse(me, "q and k overlap");
+    if(heads[1] > 0 && any && (meet(out[0], out[1]) || meet(out[0], in[1]) || meet(in[0], out[1]))) refuse(me, "q and k overlap");
+    if(any) {
+      const int64_t ps = p->positions_are_64bit ? 8 : 4;
+      if(tooFar(p->pos_batch_stride, p->batch) || tooFar(p->pos_seq_stride, p->seq) || tooFar(p->pos_axis_stride, p->axes)) refuse(me, "positions: a stride is out of range");
+      const Box pos{(const char*)p->positions, {p->batch, p->seq, p->axes}, {p->pos_batch_stride * ps, p->pos_seq_stride * ps, p->pos_axis_stride * ps}, ps};
+      const int64_t freqBytes = (int64_t)p->freq_heads * p->axes * p->pairs * 8;
+      const Box freq{(const char*)p->frequencies, {1, 1, 1}, {0, 0, 0}, freqBytes};
+      for(int i = 0; i < (heads[1] > 0 ? 2 : 1); i++)
+        if(meet(out[i], pos) || meet(out[i], freq)) refuse(me, "an output overlaps the positions or the frequencies");
     }
-    else if(heads[1] > 0 && any && (cross(out[0], out[1]) || cross(out[0], in[1]) || cross(in[0], out[1]))) refuse(me, "q and k overlap");
     a.positions = p->positions;
     a.posBatch = p->pos_batch_stride; a.posToken = p->pos_seq_stride; a.posAxis = p->pos_axis_stride; a.pos64 = p->positions_are_64bit != 0;
     a.freqs = p->frequencies; a.freqHeads = p->freq_heads; a.axes = p->axes; a.pairs = p->pairs; a.headDim = p->head_dim;

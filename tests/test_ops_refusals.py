@@ -144,7 +144,13 @@ T = capi.RotaryTensor
     (dict(q=T(MB, 2 * MB, 320, 64, -16, 320, 64, 16)), "strides"), (dict(q=T(MB, 2 * MB, 320, 64, 16, 320, 64, 15)), "overlap"),
     (dict(q=T(MB, 2 * MB, 320, 64, 16, 320, 0, 16)), "overlap"), (dict(q=T(MB, 2 * MB, 320, 64, 16, 1 << 50, 64, 16)), "range"),
     (dict(q=T(MB, MB + 32, 320, 64, 16, 320, 64, 16)), "not in itself"), (dict(q=T(MB, MB, 320, 64, 16, 320, 16, 80)), "not in itself"),
-    (dict(q=T(MB, 3 * MB, 320, 64, 16, 320, 64, 16)), "q and k overlap"), (dict(k=T(3 * MB, 2 * MB + 64, 160, 32, 16, 160, 32, 16)), "q and k overlap")])
+    (dict(q=T(MB, 3 * MB, 320, 64, 16, 320, 64, 16)), "q and k overlap"), (dict(k=T(3 * MB, 2 * MB + 64, 160, 32, 16, 160, 32, 16)), "q and k overlap"),
+    (dict(k=T(MB, 4 * MB, 160, 32, 16, 160, 32, 16), q=T(MB, MB, 320, 64, 16, 320, 64, 16)), "q and k overlap"),  # k read where q is written
+    (dict(q=T(MB, MB, 479, 96, 16, 479, 96, 16), k=T(MB + 128, MB + 128, 479, 96, 16, 479, 96, 16)), "overlap"),  # columns, but sequences meet
+    (dict(q=T(MB, MB, 480, 16, 80, 480, 16, 80), k=T(MB + 640 - 32, MB + 640 - 32, 480, 16, 80, 480, 16, 80)), "q and k overlap"),
+    (dict(positions=2 * MB + 8), "positions"), (dict(frequencies=4 * MB + 64), "positions"), (dict(positions=4 * MB + 604, positions_are_64bit=0), "positions"),
+    (dict(batch=1 << 20, seq=1 << 10, q=T(MB, 2 * MB, 1 << 39, 64, 16, 320, 64, 16)), "range"), (dict(pos_seq_stride=1 << 60), "range"),
+    (dict(q_heads=1 << 16, head_dim=1 << 16, pairs=1, k_heads=0), "channels")])
 def test_rotary_refuses(lib, kw, word):
     refused(lib, lib.kmx_rotary(9999, None, ctypes.byref(rotary_args(**kw))), "kmx_rotary", word)
 
@@ -153,7 +159,11 @@ def test_rotary_refuses(lib, kw, word):
     {}, dict(batch=0), dict(seq=0), dict(k_heads=0, k=T()), dict(freq_heads=2), dict(q=T(MB, MB, 320, 64, 16, 320, 64, 16)), dict(pos_batch_stride=0),
     dict(q=T(MB, 2 * MB, 0, 0, 0, 320, 64, 16)),  # a broadcast input
     dict(q=T(MB, 2 * MB, 320, 64, 16, 320, 16, 80)),  # heads before tokens
-    dict(q=T(MB, MB, 500, 100, 16, 500, 100, 16), k=T(MB + 128, MB + 128, 500, 100, 16, 500, 100, 16))])  # columns of one projection's rows
+    dict(q=T(MB, MB, 500, 100, 16, 500, 100, 16), k=T(MB + 128, MB + 128, 500, 100, 16, 500, 100, 16)),  # columns of one projection's rows
+    dict(q=T(MB, MB, 480, 16, 80, 480, 16, 80), k=T(MB + 640, MB + 640, 480, 16, 80, 480, 16, 80)),  # [batch, q's and k's heads, seq, dim], in place
+    dict(q_heads=2, q=T(MB, MB, 480, 96, 48, 480, 96, 48), k=T(MB + 32, MB + 32, 480, 96, 48, 480, 96, 48)),  # q, k, v side by side in each head
+    dict(q=T(MB, MB + 128, 640, 128, 16, 640, 128, 16)),  # out beside in, in the same rows
+    dict(positions=2 * MB + 1280)])  # behind q's last channel
 def test_rotary_takes(lib, kw):
     passes(lib, lib.kmx_rotary(9999, None, ctypes.byref(rotary_args(**kw))))
 
