@@ -305,38 +305,57 @@ __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
   }
 }
 
+// A launch's threads are counted in 32 bits: more rows than that go in several launches
+template <class TR>
+NormQuantArgs rowsFrom(const NormQuantArgs& a, int64_t first, int64_t most) {
+  typedef typename TR::T T;
+  NormQuantArgs b = a;
+  b.rows = a.rows - first < most ? a.rows - first : most;
+  b.x = (const T*)a.x + first * a.xStride;
+  if(a.residual != nullptr) b.residual = (const T*)a.residual + first * a.residualStride;
+  if(a.sum != nullptr) b.sum = (T*)a.sum + first * a.sumStride;
+  if(a.y != nullptr) b.y = (T*)a.y + first * a.yStride;
+  if(a.mask != nullptr) b.mask = a.mask + first;
+  if(a.codes != nullptr) b.codes = a.codes + first * a.codesStride;
+  if(a.scaleKind == SCALES_ROW) b.scales = (float*)a.scales + first;
+  if(a.scaleKind == SCALES_MX) b.scales = (uint8_t*)a.scales + first * (a.C / MX_BLOCK);
+  return b;
+}
 template <class TR, int TPR, int NCH>
-void launchRows(const NormQuantArgs& a, hipStream_t stream) {
+hipError_t launchRows(const NormQuantArgs& a, hipStream_t stream) {
   constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
-  auto kern = normQuantKernel<TR, TPR, NCH>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, stream, a);
+  constexpr int64_t MOST = (int64_t)0x7fffffff / BLOCK * RPB;
+  for(int64_t first = 0; first < a.rows; first += MOST) {
+    const NormQuantArgs b = rowsFrom<TR>(a, first, MOST);
+    if constexpr(NCH > 0) hipLaunchKernelGGL((normQuantKernel<TR, TPR, NCH>), dim3((unsigned)((b.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, stream, b);
+    else hipLaunchKernelGGL(normQuantLongKernel<TR>, dim3((unsigned)b.rows), dim3(BLOCK), 0, stream, b);
+    const hipError_t e = hipGetLastError();
+    if(e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 template <class TR>
-void launchOne(const NormQuantArgs& a, hipStream_t stream) {
+hipError_t launchOne(const NormQuantArgs& a, hipStream_t stream) {
   const int pieces = (a.C + 7) / 8;
-  if(pieces <= 16) launchRows<TR, 16, 1>(a, stream);
-  else if(pieces <= 32) launchRows<TR, 16, 2>(a, stream);
-  else if(pieces <= 64) launchRows<TR, 16, 4>(a, stream);
-  else if(pieces <= 128) launchRows<TR, 64, 2>(a, stream);
-  else if(pieces <= 256) launchRows<TR, 64, 4>(a, stream);
-  else if(pieces <= 512) launchRows<TR, 256, 2>(a, stream);
-  else if(pieces <= 1024) launchRows<TR, 256, 4>(a, stream);
-  else if(pieces <= 4096) launchRows<TR, 1024, 4>(a, stream);
-  else {
-    auto kern = normQuantLongKernel<TR>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
-  }
+  if(pieces <= 16) return launchRows<TR, 16, 1>(a, stream);
+  if(pieces <= 32) return launchRows<TR, 16, 2>(a, stream);
+  if(pieces <= 64) return launchRows<TR, 16, 4>(a, stream);
+  if(pieces <= 128) return launchRows<TR, 64, 2>(a, stream);
+  if(pieces <= 256) return launchRows<TR, 64, 4>(a, stream);
+  if(pieces <= 512) return launchRows<TR, 256, 2>(a, stream);
+  if(pieces <= 1024) return launchRows<TR, 256, 4>(a, stream);
+  if(pieces <= 4096) return launchRows<TR, 1024, 4>(a, stream);
+  return launchRows<TR, 1024, 0>(a, stream);  // (0: any length)
 }
 
 }  // namespace
 
 hipError_t launchNormQuant(int dtype, const NormQuantArgs& a, hipStream_t stream) {
   if(a.rows == 0) return hipSuccess;
-  if(dtype == DT_F16) launchOne<TraitsF16>(a, stream);
-  else if(dtype == DT_BF16) launchOne<TraitsBF16>(a, stream);
-  else if(dtype == DT_F32) launchOne<TraitsF32>(a, stream);
-  else return hipErrorInvalidValue;
-  return hipGetLastError();
+  if(dtype == DT_F16) return launchOne<TraitsF16>(a, stream);
+  if(dtype == DT_BF16) return launchOne<TraitsBF16>(a, stream);
+  if(dtype == DT_F32) return launchOne<TraitsF32>(a, stream);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace kmx

@@ -1,5 +1,9 @@
 """-m gpu: katago_amd.ops on the device against plain formulas in 64 bits (tests/ops_ref.py, with its tolerances): sizes around every kernel's borders, types,
 strides, masks, spoilt values, long offsets, streams and graphs, refusals, and the operators in a row as a transformer block uses them."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -9,6 +13,7 @@ from katago_amd import capi, ops
 from katago_amd.capi import KatamxError
 
 pytestmark = pytest.mark.gpu
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(autouse=True)
@@ -105,6 +110,23 @@ def test_rows_beyond_the_last_stay_as_they_were():
     ops.rms_norm(x, residual=x, y_out=out[2:7], sum_out=total[2:7])
     for t in (out, total):
         assert bool((t[:2] == 7).all()) and bool((t[7:] == 7).all()) and not bool((t[2:7] == 7).all(dim=1).any())
+
+
+@pytest.mark.parametrize("c,rows", [(2, 134217712 + 4099), (8200, 2097151 + 40)])
+def test_more_rows_than_a_launch_counts_threads(c, rows):
+    """256 threads for 16 rows, 1024 for one: the second launch's rows are those that a call on them alone gives"""
+    g = gen(41)
+    x = torch.empty(rows, c, device="cuda", dtype=torch.float16)
+    for at in (0, rows - 5000):
+        x[at:at + 5000].normal_(generator=g)
+    mask = torch.ones(rows, device="cuda")
+    mask[-7] = 0
+    n = ops.rms_norm(x, mask=mask, scales="row", want_y=True)
+    for part in (slice(0, 5000), slice(rows - 5000, rows)):
+        want = ops.rms_norm(x[part], mask=mask[part], scales="row", want_y=True)
+        assert torch.equal(n.y[part], want.y) and torch.equal(n.scales[part], want.scales)
+        assert torch.equal(n.codes[part].view(torch.uint8), want.codes.view(torch.uint8))
+    assert bool((n.y[-7] == 0).all()) and bool((n.y[-8] != 0).any())
 
 
 def test_masked_and_spoilt_rows():
@@ -283,6 +305,20 @@ def test_rotary_of_a_fused_projection():
     assert torch.equal(buf[..., (hq + hk) * d:], was[..., (hq + hk) * d:])
 
 
+def test_rotary_of_heads_before_tokens():
+    """[batch, heads of q, k and v, seq, dim] in one buffer, q and k in place"""
+    g = gen(42)
+    n, S, hq, hk, d = 2, 50, 4, 2, 32
+    buf = randn(n, hq + 2 * hk, S, d, g=g, t=torch.float16)
+    was = buf.clone()
+    q, k = buf[:, :hq].transpose(1, 2), buf[:, hq:hq + hk].transpose(1, 2)
+    pos, f = torch.arange(S, device="cuda"), ops.rotary_frequencies(d)[0].cuda()
+    ops.rotary(q, k, pos, f, q_out=q, k_out=k)
+    x = was[:, :hq + hk].transpose(1, 2).reshape(n * S, hq + hk, d)
+    ref.check_rotary(buf[:, :hq + hk].transpose(1, 2).reshape(x.shape), *ref.rotary(x, pos.repeat(n)[:, None], f[None, None], False))
+    assert torch.equal(buf[:, hq + hk:], was[:, hq + hk:])
+
+
 def test_rotary_inverse_is_the_gradient():
     """<R x, y> = <x, R^T y>, and R^T y against differences of <R x, y>, in fp32"""
     g = gen(12)
@@ -404,6 +440,34 @@ def test_the_current_device_and_stream_are_left_alone():
     call = lambda device: lib.kmx_quantize(device, None, capi.PREC_FP32, 1, 4, 32, x.data_ptr(), 32, codes.data_ptr(), 32, s.data_ptr())  # noqa: E731
     assert call(-1) == capi.KMX_ERR_INVALID_ARG and call(torch.cuda.device_count()) == capi.KMX_ERR_INVALID_ARG and call(0) == capi.KMX_OK
     torch.cuda.synchronize()
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """Nothing has loaded or set up the kernels when their launches are recorded: a norm, a tile of 256 x 256, a rotation"""
+    code = r"""
+import sys, torch
+sys.path.insert(0, %r)
+from katago_amd import ops
+with torch.no_grad():
+    x, m = torch.randn(8192, 256, device="cuda").half(), torch.randn(1024, 256, device="cuda").half()
+    pos, f = torch.arange(8192, device="cuda"), ops.rotary_frequencies(64)[0].cuda()
+    def run():
+        n = ops.rms_norm(x, scales="mx")
+        y = ops.linear8(n.codes, n.scales, *ops.quantize(m, "mx"))
+        return ops.rotary(y.unflatten(-1, (16, 64)), None, pos, f)[0]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, run())
+print("FIRST_OK")
+""" % REPO
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "FIRST_OK" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
 
 
 # ---- the operators in a row, and refusals ---------------------------------------------------------------------------
