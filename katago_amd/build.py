@@ -54,14 +54,67 @@ def _source_hash():
 
 STAMP = LIB + ".srchash"
 
+OPS_EXT = os.path.join(HERE, "_ops.so")
+OPS_EXT_SRC = os.path.join(CSRC, "ops_torch.cpp")
+OPS_EXT_STAMP = OPS_EXT + ".srchash"
+
+
+def _torch_dir():
+    """Where torch lies, without importing it; None where there is none (katago_amd.ops needs it, the rest does not)"""
+    import importlib.util
+
+    spec = importlib.util.find_spec("torch")
+    return list(spec.submodule_search_locations)[0] if spec is not None else None
+
+
+def _ops_extension_hash(torch_dir):
+    import hashlib
+
+    h = hashlib.sha256()
+    for p in (OPS_EXT_SRC, os.path.join(HERE, "..", "include", "katamx.h"), os.path.join(HERE, "..", "include", "katamx_ops.h"), os.path.join(torch_dir, "version.py")):
+        with open(p, "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
+
+
+def _ops_extension_up_to_date():
+    torch_dir = _torch_dir()
+    if torch_dir is None:
+        return True
+    try:
+        with open(OPS_EXT_STAMP) as f:
+            return os.path.exists(OPS_EXT) and f.read().strip() == _ops_extension_hash(torch_dir)
+    except OSError:
+        return False
+
+
+def build_ops_extension(force=False, verbose=True):
+    """csrc/ops_torch.cpp -> katago_amd/_ops.so: the part of katago_amd.ops that handles tensors (g++ and torch's headers, no HIP)"""
+    if not force and _ops_extension_up_to_date():
+        return
+    torch_dir = _torch_dir()
+    if torch_dir is None:
+        return
+    import sysconfig
+
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-I" + os.path.join(torch_dir, "include"), "-I" + sysconfig.get_paths()["include"],
+           "-o", OPS_EXT, OPS_EXT_SRC, "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building _ops.so failed:\n%s\n%s" % (r.stdout, r.stderr))
+    with open(OPS_EXT_STAMP, "w") as f:
+        f.write(_ops_extension_hash(torch_dir) + "\n")
+    if verbose:
+        print("[katago_amd.build] built", OPS_EXT, flush=True)
+
 
 def up_to_date():
-    """True when libkatamx.so exists and was built from exactly the sources in the tree. Decided by content, not by
+    """True when libkatamx.so (and the extension beside it) exists and was built from exactly the sources in the tree. Decided by content, not by
     mtimes: the object directory does not travel to the GPU box (.gpurunignore) and a copied tree's mtimes mean
     nothing, so tests (conftest) and bench.py both load the SAME shipped binary instead of one of them rebuilding it."""
     try:
         with open(STAMP) as f:
-            return os.path.exists(LIB) and f.read().strip() == _source_hash()
+            return os.path.exists(LIB) and f.read().strip() == _source_hash() and _ops_extension_up_to_date()
     except OSError:
         return False
 
@@ -86,6 +139,7 @@ def build_leaf_pump(verbose=True):
 
 
 def build(force=False, verbose=True):
+    build_ops_extension(force, verbose)
     if not force and up_to_date():
         build_leaf_pump(verbose)
         return LIB

@@ -1,5 +1,6 @@
 """-m gpu: katago_amd.ops on the device against plain formulas in 64 bits (tests/ops_ref.py, with its tolerances): sizes around every kernel's borders, types,
 strides, masks, spoilt values, long offsets, streams and graphs, refusals, and the operators in a row as a transformer block uses them."""
+import gc
 import os
 import subprocess
 import sys
@@ -512,6 +513,24 @@ def test_an_attention_sublayer_in_8_bits():
     assert bool((got[mask == 0] == 0).all())
 
 
+def test_calls_keep_nothing():
+    """Outputs are the caller's alone, also where a call is refused after some were allocated"""
+    a = block_inputs(gen(43))[0]
+    block(**a)
+    torch.cuda.synchronize()
+    gc.collect()  # (what earlier tests left in cycles)
+    before = torch.cuda.memory_allocated(), [sys.getrefcount(a[k]) for k in ("x", "w", "qw", "f")]
+    for _ in range(50):
+        block(**a)
+        with pytest.raises(KatamxError):
+            ops.rms_norm(a["x"], eps=float("nan"))
+    torch.cuda.synchronize()
+    gc.collect()
+    assert (torch.cuda.memory_allocated(), [sys.getrefcount(a[k]) for k in ("x", "w", "qw", "f")]) == before
+    with pytest.raises(TypeError):
+        ops.rms_norm(a["x"], eps="small")
+
+
 def test_no_rows():
     e = torch.empty(0, 64, device="cuda", dtype=torch.float16)
     n = ops.rms_norm(e, residual=e, scales="mx", want_y=True)
@@ -530,7 +549,7 @@ def test_refusals():
     mcodes, ms = ops.quantize(x, "mx")
     q, pos, f = torch.ones(8, 2, 32, device="cuda"), torch.zeros(8, device="cuda", dtype=i32), torch.ones(16, device="cuda").double()
     bad = [
-        lambda: ops.rms_norm(x.double()), lambda: ops.rms_norm(x.t()), lambda: ops.rms_norm(x[:, ::2]), lambda: ops.rms_norm(x, torch.ones(63, device="cuda")),
+        lambda: ops.rms_norm(torch._neg_view(x)), lambda: ops.rms_norm(x.double()), lambda: ops.rms_norm(x.t()), lambda: ops.rms_norm(x[:, ::2]), lambda: ops.rms_norm(x, torch.ones(63, device="cuda")),
         lambda: ops.rms_norm(x, torch.ones(64, device="cuda", dtype=torch.float16)), lambda: ops.rms_norm(x, torch.ones(64)), lambda: ops.rms_norm(x, residual=x[:4]),
         lambda: ops.rms_norm(x, residual=x.float()), lambda: ops.rms_norm(x, mask=torch.ones(7, device="cuda")), lambda: ops.rms_norm(x, scales="block"),
         lambda: ops.rms_norm(x[:, :40], scales="mx"), lambda: ops.rms_norm(x, sum_out=x), lambda: ops.rms_norm(x, y_out=x.float()), lambda: ops.rms_norm(x, y_out=x[:4]),
