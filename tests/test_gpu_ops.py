@@ -41,7 +41,7 @@ def uneven(rows, c, t, g, spread=1.0, pad=3, lead=1):
 
 # ---- norm -----------------------------------------------------------------------------------------------------------
 
-# around the row kernel's shapes: 8 x 16 lanes x 1, 2, 4; 64 lanes x 2, 4; 256 x 2, 4; 1024 x 4; longer rows
+# around the row kernel's shapes for few rows: 8 x 16 lanes; 64 lanes x 1, 2; 256, 512 and 1024 x 1; 1024 x 4; longer rows
 SIZES = [1, 7, 8, 96, 127, 129, 256, 384, 512, 513, 1000, 1025, 2048, 2049, 4096, 4097, 8192, 8200, 32768, 32769, 70000]
 
 
@@ -65,6 +65,21 @@ def test_rms_norm_sizes(c, dtype):
         n = ops.rms_norm(x)
         assert n.sum is None
         ref.check_y(n.y, ref.norm(x)[1])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,c", [(4097, 160), (4099, 384), (4100, 500), (1025, 1536), (1030, 2047), (513, 4096), (520, 3001), (257, 8192), (263, 5005)])
+def test_rms_norm_of_more_rows_than_lanes(rows, c, dtype):
+    """Rows of these lengths go on fewer lanes once there are more than 2^18 lanes' worth of them"""
+    g, t = gen(c), ref.TYPES[dtype]
+    x, r, w = uneven(rows, c, t, g, 3.0), uneven(rows, c, t, g, 1.0, pad=0), 1 + 0.3 * randn(c, g=g)
+    mask = (torch.arange(rows, device="cuda") % 5 != 1).float()
+    for scales in ("row", "mx") if c % 32 == 0 else ("row",):
+        n = ops.rms_norm(x, w, residual=r, mask=mask, scales=scales, want_y=True)
+        want_sum, want = ref.norm(x, w, 1e-6, None, r, mask)
+        assert torch.equal(n.sum, want_sum)
+        ref.check_y(n.y, want, None)
+        ref.check_codes(n.codes, n.scales, want, ref.norm_slack(want, None))
 
 
 def test_rms_norm_leading_dimensions_and_broadcasts():
