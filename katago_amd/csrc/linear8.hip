@@ -8,6 +8,11 @@
 //                   a few channels 400 times the others): 1/3 of an fp16 rounding at worst.
 //   fp32 outputs    the codes, times their e8m0 scale, are exact bf16 numbers (4 significant bits): v_mfma_f32_32x32x16_bf16, all sums in
 //                   fp32, at half the rate.
+//
+// Long k is bound by the matrix cores and the LDS that feeds them: 8192^3 with row scales 408 us (2690 TFLOP/s; a large library product in 8 bits
+// reaches 2330 with scales by row, 2810 with one for all), 8190 x 11008 x 4096 with scales for 32 k each 349 us (2110), the same into fp32 728 us (1015).
+// Short k is bound by a tile's other steps, which do not overlap its products: 92416 x 1152 x 384 85 us, of which the results' way out takes 38 and the
+// requests 20 (bytes alone: 49). Few rows are bound by the weights' way in: 1 x 4096 x 4096 5.1 us (3.3 TB/s).
 #include <atomic>
 
 #include "device_common.h"

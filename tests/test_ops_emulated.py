@@ -59,7 +59,7 @@ def strided(rows, c, stride, dtype, gen, spread=1.0):
     return buf[5:].reshape(rows, stride)[:, :c]
 
 
-# every shape of the row kernel (16 lanes x 1, 2, 4 rounds; 64 x 2, 4; 256 x 2, 4; 1024 x 4; the long one), tails of a piece, one channel, one row
+# the row kernel's shapes for few rows (16 lanes, 64 x 1, 2 rounds, 256, 512 and 1024 x 1, 1024 x 4; the long one), tails of a piece, one channel, one row
 @pytest.mark.parametrize("rows,c,dtype,scales,residual,masked,beta", [
     (1, 1, "fp32", "row", False, False, False), (33, 96, "fp16", "mx", True, True, False), (17, 130, "bf16", "row", True, False, True),
     (5, 384, "fp16", "row", True, True, True), (3, 511, "fp32", None, False, True, False), (6, 1024, "bf16", "mx", False, False, False),
