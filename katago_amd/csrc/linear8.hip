@@ -10,9 +10,9 @@
 //                   fp32, at half the rate.
 //
 // Long k is bound by the matrix cores and the LDS that feeds them: 8192^3 with row scales 408 us (2690 TFLOP/s; a large library product in 8 bits
-// reaches 2330 with scales by row, 2810 with one for all), 8190 x 11008 x 4096 with scales for 32 k each 349 us (2110), the same into fp32 728 us (1015).
-// Short k is bound by a tile's other steps, which do not overlap its products: 92416 x 1152 x 384 85 us, of which the results' way out takes 38 and the
-// requests 20 (bytes alone: 49). Few rows are bound by the weights' way in: 1 x 4096 x 4096 5.1 us (3.3 TB/s).
+// reaches 2330 with scales by row, 2810 with one for all), 8190 x 11008 x 4096 with scales for 32 k each 327 us (2260), the same into fp32 730 us (1010).
+// Short k is bound by what surrounds the products, whose steps overlap in part: 92416 x 1152 x 384 68 us (3.7 TB/s; bytes alone: 49). Few rows are
+// bound by the weights' way in: 1 x 4096 x 4096 5.1 us (3.3 TB/s).
 #include <atomic>
 
 #include "device_common.h"
@@ -26,6 +26,10 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef b16x8 Bf8;
 typedef u32x4 Out16 __attribute__((aligned(2)));  // 16 bytes of an output row, which starts at any element
 typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+
+// Whole lines of results go past the caches: in them they would push out a's rows, which several work-groups read, before all have read them
+// (92416 x 1152 x 384 79 -> 68 us, x 2048 138 -> 99, 8190 x 11008 x 4096 348 -> 327)
+__device__ __forceinline__ void streamOut(void* to, u32x4 v) { __builtin_nontemporal_store(v, (Out16*)to); }
 
 constexpr int KSTEP = 128;  // k of one step: a row of 128 bytes in LDS, eight pieces of 16
 constexpr int KPIECES = 8;
@@ -82,6 +86,13 @@ __device__ __forceinline__ int anew(int x) {
   return x;
 }
 hipError_t computeUnits(int device, int* n) { return hipDeviceGetAttribute(n, hipDeviceAttributeMultiprocessorCount, device); }
+#endif
+
+constexpr int CUS = 256;  // of the chip: what the choice of a kernel was measured on
+#ifdef KMX_EMULATED_HIP
+constexpr int PER_XCD = 2, SHORT_TILES = 2;  // (few rows are many)
+#else
+constexpr int PER_XCD = CUS / 8 * 2, SHORT_TILES = 10;  // linear8ShortKernel: work-groups of an XCD, tiles of each at least
 #endif
 
 template <int I> struct Index { static constexpr int value = I; };
@@ -394,7 +405,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     const unsigned mineTo = (unsigned)(ln / P) * (unsigned)g.outStride * (unsigned)sizeof(TO) + (unsigned)(ln % P) * 16;
     auto put = [&](int row0, u32x4 v) {
       TO* const to = (TO*)((char*)(corner + (int64_t)row0 * g.outStride) + mineTo);
-      if(WHOLE) *(Out16*)to = v;
+      if(WHOLE && BM > 64) streamOut(to, v);
+      else if(WHOLE) *(Out16*)to = v;  // (few rows: whatever reads them next finds them in the caches)
       else if(row0 + ln / P <= rowsLeft) {
         const int c = ln % P * PER;
         if(c + PER - 1 <= colsLeft) *(Out16*)to = v;
@@ -518,6 +530,265 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     id += gridDim.x;
     tile = next;
     tileParity ^= 1;
+  }
+  waitLoads<0>();  // (nothing may land in LDS that is another work-group's by then)
+}
+
+// Short k, many rows: a work-group keeps 128 output channels, whose weights stay in its waves' registers (64 channels of up to 384 k each), and goes down its
+// rows 128 at a time: only a's rows pass through LDS, in steps of 128 k, three of them on their way while one is multiplied. One barrier a step: behind
+// it the stage before has been read out by all and is requested anew. Two work-groups share a CU, so that one's products run beside the other's
+// results on their way out. The layouts are those of linear8Kernel; what lies beyond K has weights of zero. 92416 x 1152 x 384: 68 us (77 with linear8Kernel,
+// which fetches the weights anew for every tile), of which products alone take 39, the results' way through LDS 20; k = 128: 41 us, 5.4 TB/s.
+template <int KS, bool MX, int OUT>
+__global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int groups) {
+  typedef typename OutTraits<OUT>::TR TR;
+  typedef typename TR::T TO;
+  constexpr int BM = 128, BN = 128, NW = 4, MI = 2, NI = 2, REQ = BM / 8 / NW, STAGES = 4;
+  constexpr unsigned STAGE = BM * KSTEP;
+  HIP_DYNAMIC_SHARED(f32x4, smemLinear8)
+  const unsigned lds = ldsAddress(smemLinear8);
+  float* const scalesOf = (float*)((char*)smemLinear8 + STAGES * STAGE);  // [BN]
+  float* const biasOf = scalesOf + BN;                                    // [BN]
+  const unsigned patch = lds + STAGES * STAGE + 2 * BN * 4;               // 2 KB of each wave: what is being stored
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hh = lane >> 5;
+  const int wm = wave >> 1, wn = wave & 1;
+  const int pieces = g.K / 16, blocks = MX ? g.K / MX_BLOCK : 0;
+
+  // Work-groups go round the 8 XCDs one by one: those of an XCD that follow each other share their rows and differ in their channels, so that a's
+  // rows come from memory once
+  const unsigned mTiles = (unsigned)((g.rows + BM - 1) / BM), nTiles = (unsigned)(g.N + BN - 1) / BN;
+  const unsigned xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+  if(local >= groups * nTiles) return;
+  const int n0 = (int)(local % nTiles) * BN;
+  const unsigned group = xcd * groups + local / nTiles, allGroups = 8 * groups;
+  const unsigned first = (unsigned)((uint64_t)mTiles * group / allGroups), end = (unsigned)((uint64_t)mTiles * (group + 1) / allGroups);
+  if(first == end) return;
+  const int nLast = (g.N - n0 < BN ? g.N - n0 : BN) - 1;
+  auto lastRowOf = [&](unsigned tile) { return (int)(g.rows - (int64_t)tile * BM < BM ? g.rows - (int64_t)tile * BM : BM) - 1; };
+
+  // weights, their codes, channel scales and biases
+  u32x4 fw[KS][2][NI][2];
+  unsigned wCodes[MX ? KS : 1][NI];
+#pragma unroll
+  for(int ni = 0; ni < NI; ni++) {
+    const int c = wn * 64 + ni * 32 + col, row = n0 + (c < nLast ? c : nLast);
+    const uint8_t* const wp = g.w + (int64_t)row * g.wStride;
+#pragma unroll
+    for(int k = 0; k < KS; k++) {
+#pragma unroll
+      for(int s = 0; s < 2; s++)
+#pragma unroll
+        for(int b = 0; b < 2; b++) {
+          const int piece = k * KPIECES + 4 * s + 2 * b + hh;
+          fw[k][s][ni][b] = *(const u32x4*)(wp + (size_t)(piece < pieces ? piece : pieces - 1) * 16);
+          if(piece >= pieces) {
+#pragma unroll
+            for(int i = 0; i < 4; i++) fw[k][s][ni][b][i] = 0;
+          }
+        }
+      if constexpr(MX) wCodes[k][ni] = *(const u32u*)((const uint8_t*)g.wScales + (int64_t)row * blocks + k * 4) >> (8 * hh);
+    }
+  }
+  if(threadIdx.x < BN) {
+    const int c = (int)threadIdx.x, n = n0 + (c < nLast ? c : nLast);
+    scalesOf[c] = MX ? 1.0f : ((const float*)g.wScales)[n];
+    biasOf[c] = g.bias != nullptr ? g.bias[n] : 0.0f;
+  }
+
+  const unsigned piece = (unsigned)((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7));  // ((r >> 1) & 7 of every row that this lane requests)
+  struct Request {
+    Rsrc a;
+    unsigned in, dst;
+    int last;
+  };
+  auto requestOf = [&](unsigned at) {  // of step `at` of this work-group; beyond its last: that tile again, not used
+    const unsigned tile = first + at / KS < end ? first + at / KS : end - 1;
+    const int k = (int)(at % KS), over = k * KPIECES + (int)piece - (pieces - 1);
+    Request r;
+    r.a = bufferOf(g.a + (int64_t)tile * BM * g.aStride);
+    r.in = (unsigned)k * KSTEP + piece * 16 - (over > 0 ? (unsigned)over * 16 : 0u);
+    r.dst = lds + (at & (STAGES - 1)) * STAGE + (unsigned)wave * 8 * KSTEP;
+    r.last = lastRowOf(tile);
+    return r;
+  };
+  auto issue = [&](const Request& q, int j) {
+    const int r = (wave + NW * j) * 8 + (lane >> 3);
+    dma16(q.a, (unsigned)(r < q.last ? r : q.last) * (unsigned)g.aStride + q.in, 0, q.dst + (unsigned)(NW * j) * 8 * KSTEP);
+  };
+  constexpr int STORES = MI * 32 * 64 * (int)sizeof(TO) / 1024;  // a wave's store instructions of a whole tile
+  auto store = [&](f32x16 (&acc)[NI][MI], const float (&sa)[MI], unsigned tile, auto wholeTag) {
+    constexpr bool WHOLE = decltype(wholeTag)::value != 0;
+    constexpr int PER = 8, P = 8, ROWS = 16;
+    const unsigned mine = patch + (unsigned)wave * 2048;
+    const int ln = anew(lane), col = ln & 31, hh = ln >> 5;
+    const float* const sc = scalesOf + wn * 64;
+    const float* const bi = biasOf + wn * 64;
+    TO* const corner = (TO*)g.out + ((int64_t)tile * BM + wm * 64) * g.outStride + n0 + wn * 64;
+    const int rowsLeft = lastRowOf(tile) - wm * 64, colsLeft = nLast - wn * 64;
+    const unsigned from = mine + (unsigned)(ln / P * P + (ln % P ^ (ln / P & 7))) * 16;
+    const unsigned mineTo = (unsigned)(ln / P) * (unsigned)g.outStride * (unsigned)sizeof(TO) + (unsigned)(ln % P) * 16;
+    auto put = [&](int row0, u32x4 v) {
+      TO* const to = (TO*)((char*)(corner + (int64_t)row0 * g.outStride) + mineTo);
+      if(WHOLE && KS > 1) streamOut(to, v);
+      else if(WHOLE) *(Out16*)to = v;  // (k of 128: writing is all there is, and 92416 x 1152 take 41 us so, 47 past the caches)
+      else if(row0 + ln / P <= rowsLeft) {
+        const int c = ln % P * PER;
+        if(c + PER - 1 <= colsLeft) *(Out16*)to = v;
+        else {
+          struct Elements { TO e[PER]; };
+          const Elements e = __builtin_bit_cast(Elements, v);
+#pragma unroll
+          for(int k = 0; k < PER; k++)
+            if(c + k <= colsLeft) to[k] = e.e[k];
+        }
+      }
+    };
+    u32x4 out[MI][NI][2];  // pieces of channels 16 j + 8 hh + [0, 8)
+#pragma unroll
+    for(int ni = 0; ni < NI; ni++) {
+      u32x2 pk[MI][4];
+#pragma unroll
+      for(int q = 0; q < 4; q++) {
+        const f32x4 bias = *(const f32x4*)(bi + ni * 32 + 8 * q + 4 * hh);
+        f32x4 sw = bias;
+        if(!MX) sw = *(const f32x4*)(sc + ni * 32 + 8 * q + 4 * hh);
+#pragma unroll
+        for(int mi = 0; mi < MI; mi++) {
+          typename TR::V4 h;
+#pragma unroll
+          for(int i = 0; i < 4; i++) {
+            const float sum = acc[ni][mi][4 * q + i];
+            h[i] = TR::fromFloat((MX ? sum : sum * sa[mi] * sw[i]) + bias[i]);
+          }
+          pk[mi][q] = __builtin_bit_cast(u32x2, h);
+        }
+      }
+#pragma unroll
+      for(int mi = 0; mi < MI; mi++) pairUp(pk[mi], out[mi][ni]);
+    }
+#pragma unroll
+    for(int r0 = 0; r0 < 32 * MI; r0 += ROWS) {
+      if(col >= r0 % 32 && col < r0 % 32 + ROWS) {
+        const int r = col - r0 % 32;
+#pragma unroll
+        for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+          for(int j = 0; j < 2; j++) {
+            const int p = ni * 4 + 2 * j + hh;
+            ldsWrite16(mine + (unsigned)(r * P + (p ^ (r & 7))) * 16, out[r0 / 32][ni][j]);
+          }
+      }
+      waveFence();  // (a wave's LDS instructions are carried out in order)
+      const u32x4 v0 = ldsRead16(from), v1 = ldsRead16(from + 1024);
+      waveFence();
+      put(r0, v0);
+      put(r0 + ROWS / 2, v1);
+    }
+  };
+
+#pragma unroll
+  for(unsigned k = 0; k < 3; k++) {
+    const Request q = requestOf(k);
+#pragma unroll
+    for(int j = 0; j < REQ; j++) issue(q, j);
+  }
+  waitLoads<0>();
+  const unsigned swz = (unsigned)(col >> 1) & 7u;
+  unsigned at = 0;
+  // a's scales (or codes) are fetched a tile ahead: in front of the stores of the tile before, which a load has to wait for
+  float saNext[MI];
+  unsigned codesNext[MX ? KS : 1][MI];
+  auto fetchScales = [&](unsigned tile) {
+    const int last = lastRowOf(tile);
+#pragma unroll
+    for(int mi = 0; mi < MI; mi++) {
+      const int r = wm * 64 + mi * 32 + col;
+      const int64_t row = (int64_t)tile * BM + (r < last ? r : last);
+      saNext[mi] = MX ? 1.0f : ((const float*)g.aScales)[row];
+      if constexpr(MX) {
+#pragma unroll
+        for(int k = 0; k < KS; k++) codesNext[k][mi] = *(const u32u*)((const uint8_t*)g.aScales + row * blocks + k * 4);
+      }
+    }
+  };
+  fetchScales(first);
+  for(unsigned tile = first; tile < end; tile++) {
+    float sa[MI];
+    unsigned aCodes[MX ? KS : 1][MI];
+#pragma unroll
+    for(int mi = 0; mi < MI; mi++) {
+      sa[mi] = saNext[mi];
+      if constexpr(MX) {
+#pragma unroll
+        for(int k = 0; k < KS; k++) aCodes[k][mi] = codesNext[k][mi] >> (8 * hh);
+      }
+    }
+    f32x16 acc[NI][MI];
+#pragma unroll
+    for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+      for(int mi = 0; mi < MI; mi++)
+#pragma unroll
+        for(int v = 0; v < 16; v++) acc[ni][mi][v] = 0.0f;
+    auto step = [&](auto kTag) {
+      constexpr int k = decltype(kTag)::value;
+      // Younger than what this step multiplies are the requests of the next two and the stores of the tiles in between: a tile whose stores cannot be
+      // counted waits for all of them
+      constexpr int TILES = KS == 1 ? 3 : KS == 2 ? 2 - k : 1;
+      waitLoads<2 * REQ + TILES * STORES>();
+      waitReads0();
+      waveBarrier();
+      if constexpr(k == 0) fetchScales(tile + 1 < end ? tile + 1 : tile);
+      const Request q = requestOf(at + 3);
+      const unsigned rows = lds + (at & (STAGES - 1)) * STAGE + (unsigned)(wm * 64 + col) * KSTEP;
+      u32x4 fa[MI][2][2];
+#pragma unroll
+      for(int mi = 0; mi < MI; mi++)
+#pragma unroll
+        for(int s = 0; s < 2; s++)
+#pragma unroll
+          for(int b = 0; b < 2; b++) fa[mi][s][b] = ldsRead16(rows + mi * 32 * KSTEP + (((unsigned)(4 * s + 2 * b + hh)) ^ swz) * 16);
+#pragma unroll
+      for(int mi = 0; mi < MI; mi++)
+#pragma unroll
+        for(int s = 0; s < 2; s++)
+#pragma unroll
+          for(int ni = 0; ni < NI; ni++) {
+            constexpr int UNIT = 0x7f7f7f7f;
+            i32x8 xa, xw;
+#pragma unroll
+            for(int i = 0; i < 8; i++) {
+              xa[i] = (int)fa[mi][s][i >> 2][i & 3];
+              xw[i] = (int)fw[k][s][ni][i >> 2][i & 3];
+            }
+            if(s == 0)
+              acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw, xa, acc[ni][mi], 0, 0, 0, MX ? (int)wCodes[MX ? k : 0][ni] : UNIT, 0,
+                                                                            MX ? (int)aCodes[MX ? k : 0][mi] : UNIT);
+            else
+              acc[ni][mi] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xw, xa, acc[ni][mi], 0, 0, 2, MX ? (int)wCodes[MX ? k : 0][ni] : UNIT, 2,
+                                                                            MX ? (int)aCodes[MX ? k : 0][mi] : UNIT);
+            if(ni == NI - 1) {  // (requests hold a wave's issue for as long as a product takes: one after two of them)
+              __builtin_amdgcn_sched_barrier(0);
+              issue(q, mi * 2 + s);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+      static_assert(REQ == 2 * MI, "a request to each half's products");
+#pragma unroll
+      for(int ni = 0; ni < NI; ni++)
+#pragma unroll
+        for(int mi = 0; mi < MI; mi++) computed(acc[ni][mi]);
+      at++;
+    };
+    step(Index<0>());
+    if constexpr(KS > 1) step(Index<1>());
+    if constexpr(KS > 2) step(Index<2>());
+    if(lastRowOf(tile) == BM - 1 && nLast == BN - 1) store(acc, sa, tile, Index<1>());
+    else {
+      store(acc, sa, tile, Index<0>());
+      waitLoads<0>();
+    }
   }
   waitLoads<0>();  // (nothing may land in LDS that is another work-group's by then)
 }
@@ -649,6 +920,25 @@ hipError_t launchFew(const Linear8Args& g, hipStream_t stream) {
   hipLaunchKernelGGL(kern, dim3((unsigned)((g.N + 15) / 16), (unsigned)((g.rows + 16 * MT - 1) / (16 * MT))), dim3(512), 0, stream, g);
   return hipGetLastError();
 }
+// The current device's compute units, asked for once per instantiation and device (cus: 0 until then); a kernel's large LDS window is opted in to there
+constexpr int MAX_DEVICES = 64;
+template <class K>
+hipError_t prepared(K kern, int lds, std::atomic<int>* cus, int* n) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if(e != hipSuccess) return e;
+  if(dev < 0 || dev >= MAX_DEVICES) return hipErrorInvalidDevice;
+  *n = cus[dev].load(std::memory_order_acquire);
+  if(*n != 0) return hipSuccess;
+  if(lds > 64 * 1024) {
+    e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if(e != hipSuccess) return e;
+  }
+  e = computeUnits(dev, n);
+  if(e != hipSuccess) return e;
+  cus[dev].store(*n, std::memory_order_release);
+  return hipSuccess;
+}
 template <int BM, int BN, int WM, int WN, int STAGES, bool MX, int OUT>
 hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const int64_t tiles = (g.rows + BM - 1) / BM * ((g.N + BN - 1) / BN);
@@ -657,24 +947,23 @@ hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   constexpr int PER_CU = ALL_LDS / LDS < 4 ? ALL_LDS / LDS : 4;  // work-groups of a CU
   static_assert(PER_CU >= 1, "LDS");
   auto kern = linear8Kernel<BM, BN, WM, WN, STAGES, MX, OUT>;
-  constexpr int MAX_DEVICES = 64;
-  static std::atomic<int> cus[MAX_DEVICES];  // 0: not asked yet
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
+  static std::atomic<int> cus[MAX_DEVICES];
+  int n = 0;
+  const hipError_t e = prepared(kern, LDS, cus, &n);
   if(e != hipSuccess) return e;
-  if(dev < 0 || dev >= MAX_DEVICES) return hipErrorInvalidDevice;
-  int n = cus[dev].load(std::memory_order_acquire);
-  if(n == 0) {  // once per instantiation and device
-    if(LDS > 64 * 1024) {  // opt in to the large LDS window
-      e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-      if(e != hipSuccess) return e;
-    }
-    e = computeUnits(dev, &n);
-    if(e != hipSuccess) return e;
-    cus[dev].store(n, std::memory_order_release);
-  }
   const int64_t most = (int64_t)n * PER_CU / 8 * 8;  // (a multiple of the XCDs: a work-group's tiles stay on its XCD's part)
   hipLaunchKernelGGL(kern, dim3((unsigned)(tiles < most ? tiles : most)), dim3(64 * WM * WN), LDS, stream, g);
+  return hipGetLastError();
+}
+template <int KS, bool MX, int OUT>
+hipError_t launchShort(const Linear8Args& g, int groups, hipStream_t stream) {
+  constexpr int LDS = 4 * 128 * KSTEP + 2 * 128 * 4 + 4 * 2048;
+  auto kern = linear8ShortKernel<KS, MX, OUT>;
+  static std::atomic<int> cus[MAX_DEVICES];
+  int n = 0;
+  const hipError_t e = prepared(kern, LDS, cus, &n);
+  if(e != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(8 * groups * ((g.N + 127) / 128))), dim3(256), LDS, stream, g, groups);
   return hipGetLastError();
 }
 template <bool MX, int OUT>
@@ -682,6 +971,16 @@ hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
   // Few rows: up to 32 on the kernel without LDS (32 x 4096 x 4096 8.1 us; 64 rows 11.7 against 10.0 on 64 x 64 tiles with four stages), up to 64 where k
   // is too short for those to get going (64 x 1152 x 384 3.0 us against 3.8).
   const bool longK = g.K >= 8 * KSTEP;
+  // k that fits the registers, and rows enough: ten tiles of 128 rows to a work-group (12.9 of them, 92416 x 1152 x 384: 68 us against 77; 11.3, n = 1024:
+  // equal; 4.3, n = 384: 28 against 26.7; two, 14500 x 1152: 18.7 against 15.4)
+  if constexpr(OUT != DT_F32) {
+    const int64_t groups = PER_XCD / ((g.N + 127) / 128);  // of work-groups that share their rows, on an XCD
+    if(g.K <= 3 * KSTEP && (!MX || g.K % KSTEP == 0) && groups >= 1 && (g.rows + 127) / 128 >= SHORT_TILES * 8 * groups) {
+      if(g.K <= KSTEP) return launchShort<1, MX, OUT>(g, (int)groups, stream);
+      if(g.K <= 2 * KSTEP) return launchShort<2, MX, OUT>(g, (int)groups, stream);
+      return launchShort<3, MX, OUT>(g, (int)groups, stream);
+    }
+  }
   if(g.rows <= 16) return launchFew<1, MX, OUT>(g, stream);
   if(g.rows <= 32) return launchFew<2, MX, OUT>(g, stream);
   if(g.rows <= 64 && !longK) return launchFew<4, MX, OUT>(g, stream);
@@ -690,7 +989,7 @@ hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
   // k = 384: n = 1152 in 84 us against 89, but n = 384, half of its second tile empty, in 34 against 28); the small one while there is a
   // round of it - with one work-group to a CU four stages, which hide a request's time better (1000 x 4096 x 4096 27.1 -> 24.0 us);
   // below that 64 x 64, with four stages where k is long (128 x 4096 x 4096 16.8 -> 10.0 us, 361 x 1152 x 384 3.8 -> 4.9).
-  const int64_t cus = 256;
+  const int64_t cus = CUS;
   auto tiles = [&](int b) { return (g.rows + b - 1) / b * ((g.N + b - 1) / b); };
   const int64_t large = tiles(256), small = tiles(128);
   if constexpr(OUT != DT_F32)

@@ -196,6 +196,24 @@ def eight(rows, k, scales, g, spread=1.0):
     return ops.quantize(randn(rows, k, g=g, spread=spread), scales)
 
 
+@pytest.mark.parametrize("out", ["fp16", "bf16"])
+@pytest.mark.parametrize("scales", ["row", "mx"])
+@pytest.mark.parametrize("m,n,k", [(655400, 100, 288), (655360, 128, 384), (330001, 256, 128), (327000, 130, 256), (217100, 384, 352), (72500, 1152, 384), (71680, 1100, 32),
+                                   (92416, 1152, 384), (10300, 8192, 256), (10240, 8065, 384), (10111, 8192, 96), (10305, 8192, 128), (72449, 1152, 256)])
+def test_linear8_of_many_rows_and_short_k(m, n, k, scales, out):
+    """The kernel that keeps its weights: whole tiles and partial ones, channels for one work-group to sixty-four, rows around the fewest that it takes"""
+    g = gen(m + n)
+    a, sa = eight(m, k, scales, g)
+    w, sw = eight(n, k, scales, g)
+    b = randn(n, g=g) if n % 3 else None
+    buf = torch.full((m, n + 9), 7.0, device="cuda", dtype=ref.TYPES[out])
+    y = ops.linear8(a, sa, w, sw, b, out=buf[:, 1:n + 1])
+    for lo in range(0, m, 20000):
+        part = slice(lo, min(m, lo + 20000))
+        ref.check_linear(y[part], *ref.linear(ref.values(a[part], sa[part]), ref.values(w, sw), b), k)
+    assert bool((buf[:, 0] == 7).all()) and bool((buf[:, n + 1:] == 7).all())
+
+
 @pytest.mark.parametrize("out", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("scales", ["row", "mx"])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 4096, 4096), (2, 100, 96), (16, 1000, 512), (17, 64, 2048), (33, 33, 64), (361, 1152, 384), (64, 65, 128),

@@ -175,7 +175,10 @@ def aligned_copy(codes, stride):
     (1, 1, 32, "mx", "fp32", False), (1, 40, 16, "row", "bf16", True), (70, 33, 144, "row", "fp16", True), (65, 72, 160, "mx", "bf16", False),
     (64, 64, 128, "row", "fp32", True), (66, 64, 128, "row", "fp32", True), (16, 17, 1168, "row", "bf16", True), (3, 16, 4128, "mx", "fp16", False),
     (20, 30, 1056, "mx", "fp32", True), (64, 20, 2064, "row", "fp16", False), (70, 20, 96, "mx", "bf16", False),
-    (65, 66, 1168, "row", "fp16", True), (70, 130, 1056, "mx", "bf16", True), (300, 70, 1040, "row", "fp32", False), (9, 130, 288, "mx", "fp32", True), (130, 8, 272, "row", "fp16", False), (33, 64, 256, "mx", "fp16", True)])
+    (65, 66, 1168, "row", "fp16", True), (70, 130, 1056, "mx", "bf16", True), (300, 70, 1040, "row", "fp32", False), (9, 130, 288, "mx", "fp32", True), (130, 8, 272, "row", "fp16", False), (33, 64, 256, "mx", "fp16", True),
+    # rows enough (here) for the kernel that keeps its weights: one, two, three steps of k, whole tiles and partial ones, one and two tiles of channels
+    (4230, 100, 272, "row", "fp16", True), (4096, 128, 384, "mx", "bf16", True), (2100, 200, 128, "mx", "fp16", False), (2300, 256, 256, "row", "bf16", True),
+    (4097, 128, 16, "row", "fp16", True), (4352, 128, 384, "row", "fp16", True)])
 def test_linear8(emu, m, n, k, scales, out, bias):
     g = torch.Generator().manual_seed(m * 1000 + n)
     a, sa = eight(m, k, scales, g, 2.0)
