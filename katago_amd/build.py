@@ -97,11 +97,13 @@ def build_ops_extension(force=False, verbose=True):
         return
     import sysconfig
 
+    fresh = "%s.%d" % (OPS_EXT, os.getpid())  # (moved into place whole: several test workers may build at once)
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-I" + os.path.join(torch_dir, "include"), "-I" + sysconfig.get_paths()["include"],
-           "-o", OPS_EXT, OPS_EXT_SRC, "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+           "-o", fresh, OPS_EXT_SRC, "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("building _ops.so failed:\n%s\n%s" % (r.stdout, r.stderr))
+    os.replace(fresh, OPS_EXT)
     with open(OPS_EXT_STAMP, "w") as f:
         f.write(_ops_extension_hash(torch_dir) + "\n")
     if verbose:
