@@ -9,7 +9,7 @@
 // Everything between the loads and the stores is fp32. e4m3 rounds to nearest even: 448 is its largest value, nothing clips.
 //
 // Bound by memory: a row's values stay in registers, so that everything is read once and written once. 92416 rows of 384 channels in fp16 with residual,
-// mask and codes 49 us (5.1 TB/s; a large copy reaches 5.1), 8190 of 4096 in bf16 with sum, y and codes for 32 channels each 57 us (5.3), the
+// mask and codes 51 us (4.9 TB/s; a large copy reaches 5.1), 8190 of 4096 in bf16 with sum, y and codes for 32 channels each 56 us (5.4), the
 // 8-bit form alone of 16383 x 1536 15.6 us (4.9). A few rows are bound by one trip to memory and a launch: 361 x 384 3.3 us.
 #include "device_common.h"
 #include "ops.h"
@@ -162,13 +162,28 @@ __device__ __forceinline__ unsigned rowMax(unsigned v, unsigned* part) {
   return v;
 }
 
-// The norm's factor applied to 8 values: v * r * w + beta, 0 on a masked row
-__device__ __forceinline__ void scale8(const NormQuantArgs& a, int c, float r, bool on, float (&v)[8]) {
+// 1 / sqrt(sum / C + eps) in two parts: fp32's own error in it (up to 2^-23) would be the row's in every channel and move codes and scales that lie next
+// to a border. One Newton step on what is left of 1 - x r^2; a sum that overflowed gives 0, a row of zeros without eps infinity, both without a second part.
+struct Factor {
+  float hi, lo;
+};
+__device__ __forceinline__ Factor factorOf(const NormQuantArgs& a, float sum) {
+  const double x = (double)sum * a.perChannel + (double)a.eps;
+  const float xh = (float)x, xl = (float)(x - (double)xh), r = rsqrtf(xh);
+  const float t = xh * r, left = __builtin_fmaf(-t, r, 1.0f) - (__builtin_fmaf(xh, r, -t) + xl * r) * r, lo = 0.5f * r * left;
+  return Factor{r, __builtin_fabsf(lo) < r * 1e-3f ? lo : 0.0f};
+}
+// The norm's factor applied to 8 values: v * r * w, rounded once, + beta; 0 on a masked row. (Of 33.5 million codes 8 lie on the other side of a border than
+// the formula's in 64 bits; 15 with fp32's root and each product rounded. 256 boards take 1.3 us longer for it.)
+__device__ __forceinline__ void scale8(const NormQuantArgs& a, int c, Factor r, bool on, float (&v)[8]) {
   if(!a.normed) return;
   float w[8];
   if(a.weight != nullptr) load8<TraitsF32>(a.weight, c, a.C, w);
 #pragma unroll
-  for(int i = 0; i < 8; i++) v[i] = v[i] * r * (a.weight != nullptr ? w[i] : 1.0f);
+  for(int i = 0; i < 8; i++) {
+    const float p = v[i] * r.hi, e = __builtin_fmaf(v[i], r.lo, __builtin_fmaf(v[i], r.hi, -p));
+    v[i] = a.weight != nullptr ? __builtin_fmaf(p, w[i], e * w[i]) : p + e;
+  }
   if(a.beta != nullptr) {
     load8<TraitsF32>(a.beta, c, a.C, w);
 #pragma unroll
@@ -223,8 +238,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void normQuantKernel(NormQua
 #pragma unroll
     for(int j = 0; j < 8; j++) ss += v[i][j] * v[i][j];
   }
-  float r = 1.0f;
-  if(a.normed) r = rsqrtf(rowSum<TPR>(ss, part[0]) / (float)a.C + a.eps);
+  Factor r = {1.0f, 0.0f};
+  if(a.normed) r = factorOf(a, rowSum<TPR>(ss, part[0]));
   const bool on = a.mask == nullptr || !valid || a.mask[row] != 0.0f;
   unsigned top = 0;
 #pragma unroll
@@ -271,7 +286,7 @@ __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
   const int64_t row = blockIdx.x;
   const T* const h = a.residual != nullptr ? (const T*)a.sum + row * a.sumStride : (const T*)a.x + row * a.xStride;
   float v[8];
-  float r = 1.0f;
+  Factor r = {1.0f, 0.0f};
   if(a.normed) {
     float ss = 0.0f;
     for(int c = threadIdx.x * 8; c < a.C; c += TPR * 8) {
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
 #pragma unroll
       for(int j = 0; j < 8; j++) ss += v[j] * v[j];
     }
-    r = rsqrtf(rowSum<TPR>(ss, part[0]) / (float)a.C + a.eps);
+    r = factorOf(a, rowSum<TPR>(ss, part[0]));
   }
   const bool on = a.mask == nullptr || a.mask[row] != 0.0f;
   float scale = 1.0f, inv = 1.0f;

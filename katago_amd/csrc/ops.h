@@ -29,6 +29,7 @@ struct NormQuantArgs {
   int scaleKind;
   int normed;  // 0: the 8-bit form of x alone
   float eps;
+  double perChannel;  // 1 / C
 };
 hipError_t launchNormQuant(int dtype, const NormQuantArgs& a, hipStream_t stream);
 

@@ -167,7 +167,7 @@ int kmx_rmsnorm(int device, void* stream, const kmx_rmsnorm_args* p) {
     a.x = p->x; a.residual = p->residual; a.sum = p->sum; a.weight = p->weight; a.beta = p->beta; a.mask = p->mask; a.y = p->y;
     a.codes = (uint8_t*)p->codes; a.scales = p->scales;
     a.xStride = p->x_stride; a.residualStride = p->residual_stride; a.sumStride = p->sum_stride; a.yStride = p->y_stride; a.codesStride = p->codes_stride;
-    a.rows = n; a.C = p->channels; a.scaleKind = p->scale_kind; a.normed = 1; a.eps = p->epsilon;
+    a.rows = n; a.C = p->channels; a.scaleKind = p->scale_kind; a.normed = 1; a.eps = p->epsilon; a.perChannel = 1.0 / p->channels;
     OnDevice on(device);
     hipCheck(launchNormQuant(dtype, a, (hipStream_t)stream), "rmsnorm launch");
   });

@@ -32,7 +32,7 @@ def norm(x, w=None, eps=1e-6, beta=None, residual=None, mask=None):
 
 def norm_slack(y, beta=None):
     """How far fp32 arithmetic may bring y from y: the sum of squares adds at most 40 terms one after the other, then 10 levels of a tree (50 U, half
-    of it in the root), the root's instruction 2 U, three products: under 32 U of the product, one more of the sum with beta."""
+    of it in the root), the root and the products 3 U: under 32 U of the product, one more of the sum with beta."""
     b = 0.0 if beta is None else beta.double().abs()
     return 40 * U * (y.abs() + 2 * b)
 
