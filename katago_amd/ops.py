@@ -20,8 +20,6 @@ from . import capi
 from .capi import KatamxError
 
 SCALES = {None: 0, "row": 1, "mx": 2}
-MX_BLOCK = 32
-E4M3_MAX = 448.0
 
 Normed = collections.namedtuple("Normed", ["sum", "y", "codes", "scales"])
 
