@@ -46,6 +46,7 @@ template <int N> inline void waitLoads() { emu::waitVm(N); }
 inline void waitReads0() {}
 inline void waveBarrier() { __syncthreads(); }
 inline int anew(int x) { return x; }
+inline void countedStore() { emu::vmNote(); }
 template <class V> inline void computed(V&) {}
 inline hipError_t computeUnits(int, int* n) {
   *n = 8;  // (few: work-groups go round more than once)
@@ -80,6 +81,8 @@ template <class V>
 __device__ __forceinline__ void computed(V& v) {
   asm volatile("" : "+v"(v));
 }
+// A store instruction that a later wait's count includes (the emulation enters it into the wave's queue)
+__device__ __forceinline__ void countedStore() {}
 // x, as far as the compiler can tell a new value each time: what is computed from it is not kept in registers around a loop
 __device__ __forceinline__ int anew(int x) {
   asm volatile("" : "+v"(x));
@@ -404,6 +407,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     const unsigned from = mine + (unsigned)(ln / P * P + (ln % P ^ (ln / P & SWZ))) * 16;
     const unsigned mineTo = (unsigned)(ln / P) * (unsigned)g.outStride * (unsigned)sizeof(TO) + (unsigned)(ln % P) * 16;
     auto put = [&](int row0, u32x4 v) {
+      if(WHOLE) countedStore();
       TO* const to = (TO*)((char*)(corner + (int64_t)row0 * g.outStride) + mineTo);
       if(WHOLE && BM > 64) streamOut(to, v);
       else if(WHOLE) *(Out16*)to = v;  // (few rows: whatever reads them next finds them in the caches)
@@ -629,6 +633,7 @@ __global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int 
     const unsigned from = mine + (unsigned)(ln / P * P + (ln % P ^ (ln / P & 7))) * 16;
     const unsigned mineTo = (unsigned)(ln / P) * (unsigned)g.outStride * (unsigned)sizeof(TO) + (unsigned)(ln % P) * 16;
     auto put = [&](int row0, u32x4 v) {
+      if(WHOLE) countedStore();
       TO* const to = (TO*)((char*)(corner + (int64_t)row0 * g.outStride) + mineTo);
       if(WHOLE && KS > 1) streamOut(to, v);
       else if(WHOLE) *(Out16*)to = v;  // (k of 128: writing is all there is, and 92416 x 1152 take 41 us so, 47 past the caches)

@@ -120,6 +120,11 @@ long integer(PyObject* o) {
   if(v == -1 && PyErr_Occurred()) throw PythonError();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if(v < 0) throw PythonError();
+  return v == 1;
+}
 void* currentStream(int device) {
   PyObject* const index = PyLong_FromLong(device);
   if(index == nullptr) throw PythonError();
@@ -173,7 +178,7 @@ PyObject* rmsNorm(PyObject* const* args, Py_ssize_t n) {
   const Arg x = tensor("x", args[0]), weight = tensor("weight", args[1]), beta = tensor("beta", args[3]), residual = tensor("residual", args[4]);
   const Arg mask = tensor("mask", args[5]), sumOut = tensor("sum_out", args[8]), yOut = tensor("y_out", args[9]);
   const int kind = (int)integer(args[6]);
-  const bool wantY = args[7] == Py_None ? kind == KMX_SCALES_NONE || yOut.given() : PyObject_IsTrue(args[7]) == 1;
+  const bool wantY = args[7] == Py_None ? kind == KMX_SCALES_NONE || yOut.given() : truth(args[7]);
   kmx_rmsnorm_args a = {};
   a.epsilon = (float)number(args[2]);
   if(!x.given()) refuse("x must be a tensor");
@@ -309,9 +314,9 @@ PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
   for(const Arg* a : {&q, &positions, &freqs})
     if(!a->given()) refuse(std::string(a->name) + " must be a tensor");
   kmx_rotary_args a = {};
-  a.half = PyObject_IsTrue(args[4]) == 1;
+  a.half = truth(args[4]);
   a.magnitude = (float)number(args[5]);
-  a.inverse = PyObject_IsTrue(args[6]) == 1;
+  a.inverse = truth(args[6]);
   const int device = onDevice({&q, &k, &positions, &freqs, &qOut, &kOut});
   a.type = typeOf("q", q->scalar_type());
   const int64_t lead = q->dim() - 2;

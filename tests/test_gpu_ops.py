@@ -562,6 +562,8 @@ def test_calls_keep_nothing():
     assert (torch.cuda.memory_allocated(), [sys.getrefcount(a[k]) for k in ("x", "w", "qw", "f")]) == before
     with pytest.raises(TypeError):
         ops.rms_norm(a["x"], eps="small")
+    with pytest.raises(RuntimeError):
+        ops.rms_norm(a["x"], want_y=torch.ones(2))  # (has no truth value)
 
 
 def test_no_rows():

@@ -4,6 +4,7 @@ stay as they were. What the hardware adds is tests/test_gpu_ops.py's part."""
 import ctypes
 import os
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -193,6 +194,27 @@ def test_linear8(emu, m, n, k, scales, out, bias):
     want, mag = ref.linear(ref.values(a, sa), ref.values(w, sw), b)
     ref.check_linear(y.get(), want, mag, k)
     y.rest_untouched()
+
+
+@pytest.mark.parametrize("mode", ["1", "2"])
+def test_linear8_copies_as_late_as_the_waits_allow(emu, mode):
+    """The same with every copy into LDS landing only when a wait requires it (1), or at the barrier behind that wait (2), the counted stores of a tile among the
+    requests: work-groups that go round several tiles, whole ones and partial ones, two stages and four, and the kernel that keeps its weights"""
+    code = r"""
+import ctypes, sys
+sys.path[:0] = [%r, %r]
+import test_ops_emulated as t
+lib = ctypes.CDLL(%r)
+t.capi.bind_ops(lib)
+lib.kmx_last_error.restype = ctypes.c_char_p
+for case in [(384, 384, 160, "row", "fp16", True), (390, 384, 288, "mx", "bf16", False), (320, 384, 1152, "row", "bf16", False), (200, 200, 1056, "mx", "fp16", True),
+             (384, 384, 256, "row", "fp32", False), (4352, 128, 384, "row", "fp16", True), (4100, 128, 256, "mx", "bf16", False), (2100, 200, 128, "row", "fp16", False)]:
+    print(case, flush=True)
+    t.test_linear8(lib, *case)
+print("LATE_OK")
+""" % (REPO, os.path.join(REPO, "tests"), emu._name)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=dict(os.environ, KMX_EMU_LATE_DMA=mode))
+    assert r.returncode == 0 and "LATE_OK" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
 
 
 def rotary_args(q, k, qo, ko, pos, f, dtype, half, magnitude, inverse):
