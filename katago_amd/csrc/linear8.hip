@@ -48,6 +48,14 @@ inline void waveBarrier() { __syncthreads(); }
 inline int anew(int x) { return x; }
 inline void countedStore() { emu::vmNote(); }
 template <class V> inline void computed(V&) {}
+inline bool anyLane(bool x) {
+  float v = x ? 1.0f : 0.0f;
+  for(int o = 1; o < 64; o <<= 1) {
+    const float u = __shfl_xor(v, o);
+    v = u > v ? u : v;
+  }
+  return v != 0.0f;
+}
 inline hipError_t computeUnits(int, int* n) {
   *n = 8;  // (few: work-groups go round more than once)
   return hipSuccess;
@@ -83,6 +91,7 @@ __device__ __forceinline__ void computed(V& v) {
 }
 // A store instruction that a later wait's count includes (the emulation enters it into the wave's queue)
 __device__ __forceinline__ void countedStore() {}
+__device__ __forceinline__ bool anyLane(bool x) { return __builtin_amdgcn_ballot_w64(x) != 0; }
 // x, as far as the compiler can tell a new value each time: what is computed from it is not kept in registers around a loop
 __device__ __forceinline__ int anew(int x) {
   asm volatile("" : "+v"(x));
@@ -115,6 +124,17 @@ __device__ __forceinline__ Bf8 bf16Of(unsigned lo, unsigned hi, float scale) {
 }
 __device__ __forceinline__ float ofE8m0(unsigned code) {  // 2^(code - 127); 0 is a denormal fp32, 255 a NaN
   return __builtin_bit_cast(float, code == 0 ? 0x00400000u : code == 255 ? 0x7fc00000u : code << 23);
+}
+
+// A sum of products of codes is 0 or between 2^-18 (the smallest product) and 2^41 (448^2 over 2^23 channels): scales between 2^-40 and 2^40 may be
+// applied one after the other and nothing leaves fp32 on the way. Of any others the mantissas are multiplied and the exponents added, so that a result
+// is infinite or below the smallest number only where the formula's is. (The choice is made once a wave and tile; 361 x 1152 x 384 take 0.15 us longer for
+// the second way's code, large products nothing.)
+__device__ __forceinline__ bool mild(float scale) { return scale >= 0x1p-40f && scale <= 0x1p40f; }
+__device__ __forceinline__ float scaledByAny(float sum, float sa, float sw) {
+  int ea, ew;
+  const float ma = frexpf(sa, &ea), mw = frexpf(sw, &ew);
+  return ldexpf(sum * ma * mw, ea + ew);
 }
 
 typedef unsigned u32u __attribute__((aligned(1)));
@@ -392,8 +412,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
   // Scales, bias, the output's type, and the way to memory: some rows at a time through 2 KB of the wave's own, so that a store instruction covers whole
   // lines (16 bytes a lane straight from the accumulators' layout: 4 % slower at 92416 x 1152 x 384). Element v of a lane: channel
   // 8 (v / 4) + 4 hh + v % 4 of the 32, row `col`; piece p of 16 bytes of a row lies at p ^ (row & SWZ). A tile that is whole has no branch here.
-  auto store = [&](const Tile& t, int parity, auto wholeTag) {
-    constexpr bool WHOLE = decltype(wholeTag)::value != 0;
+  // anyTag: scales of any size.
+  auto store = [&](const Tile& t, int parity, auto wholeTag, auto anyTag) {
+    constexpr bool WHOLE = decltype(wholeTag)::value != 0, ANY = decltype(anyTag)::value != 0;
     constexpr int PER = 16 / (int)sizeof(TO), P = TN / PER, ROWS = 2048 / (P * 16);  // elements of a piece, pieces of a row, rows of a patch
     constexpr int SWZ = (P < ROWS / 2 ? P : ROWS / 2) - 1 < 7 ? (P < ROWS / 2 ? P : ROWS / 2) - 1 : 7;
     static_assert(ROWS >= 8 && ROWS <= 32 && (P & (P - 1)) == 0, "patch");
@@ -436,7 +457,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
           f32x4 sw = bias, o;
           if(!MX) sw = *(const f32x4*)(sc + BM + wn * TN + ni * 32 + 8 * q + 4 * hh);
 #pragma unroll
-          for(int i = 0; i < 4; i++) o[i] = (MX ? acc[ni][mi][4 * q + i] : acc[ni][mi][4 * q + i] * sa * sw[i]) + bias[i];
+          for(int i = 0; i < 4; i++) {
+            const float sum = acc[ni][mi][4 * q + i];
+            o[i] = (MX ? sum : ANY ? scaledByAny(sum, sa, sw[i]) : sum * sa * sw[i]) + bias[i];
+          }
           if constexpr(OUT == DT_F32) out[ni][q] = __builtin_bit_cast(u32x4, o);
           else {
             typename TR::V4 h;
@@ -474,6 +498,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
   };
   constexpr int STORES = MI * TN * 32 * (int)sizeof(TO) / 1024;  // a wave's store instructions of a whole tile
   static_assert(STORES <= 63, "vmcnt");
+  auto allMild = [&](int parity) {  // of the scales that this wave's part is multiplied with
+    if(MX) return true;
+    const float* const sc = scalesOf + parity * (BM + BN);
+    bool ok = true;
+#pragma unroll
+    for(int r = lane; r < TM; r += 64) ok = mild(sc[wm * TM + r]) && ok;
+#pragma unroll
+    for(int c = lane; c < TN; c += 64) ok = mild(sc[BM + wn * TN + c]) && ok;
+    return !anyLane(!ok);
+  };
 
   unsigned id = blockIdx.x;
   Tile tile = tileAt(id);
@@ -525,9 +559,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     body(at++, step, STAGES - 2, step + 1, 0, Index<END>(), Index<0>());
     putScales(tileParity ^ 1);
     body(at++, step + 1, STAGES - 1, 0, 1, Index<END>(), Index<0>());
-    if(tile.mLast == BM - 1 && tile.nLast == BN - 1) store(tile, tileParity, Index<1>());
+    const bool plain = allMild(tileParity);
+    if(plain && tile.mLast == BM - 1 && tile.nLast == BN - 1) store(tile, tileParity, Index<1>(), Index<0>());
     else {
-      store(tile, tileParity, Index<0>());
+      if(plain) store(tile, tileParity, Index<0>(), Index<0>());
+      else store(tile, tileParity, Index<0>(), Index<1>());
       waitLoads<0>();  // (who knows how many of its lanes had something to store)
     }
     if(last) break;
@@ -621,8 +657,8 @@ __global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int 
     dma16(q.a, (unsigned)(r < q.last ? r : q.last) * (unsigned)g.aStride + q.in, 0, q.dst + (unsigned)(NW * j) * 8 * KSTEP);
   };
   constexpr int STORES = MI * 32 * 64 * (int)sizeof(TO) / 1024;  // a wave's store instructions of a whole tile
-  auto store = [&](f32x16 (&acc)[NI][MI], const float (&sa)[MI], unsigned tile, auto wholeTag) {
-    constexpr bool WHOLE = decltype(wholeTag)::value != 0;
+  auto store = [&](f32x16 (&acc)[NI][MI], const float (&sa)[MI], unsigned tile, auto wholeTag, auto anyTag) {
+    constexpr bool WHOLE = decltype(wholeTag)::value != 0, ANY = decltype(anyTag)::value != 0;
     constexpr int PER = 8, P = 8, ROWS = 16;
     const unsigned mine = patch + (unsigned)wave * 2048;
     const int ln = anew(lane), col = ln & 31, hh = ln >> 5;
@@ -664,7 +700,7 @@ __global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int 
 #pragma unroll
           for(int i = 0; i < 4; i++) {
             const float sum = acc[ni][mi][4 * q + i];
-            h[i] = TR::fromFloat((MX ? sum : sum * sa[mi] * sw[i]) + bias[i]);
+            h[i] = TR::fromFloat((MX ? sum : ANY ? scaledByAny(sum, sa[mi], sw[i]) : sum * sa[mi] * sw[i]) + bias[i]);
           }
           pk[mi][q] = __builtin_bit_cast(u32x2, h);
         }
@@ -789,9 +825,17 @@ __global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int 
     step(Index<0>());
     if constexpr(KS > 1) step(Index<1>());
     if constexpr(KS > 2) step(Index<2>());
-    if(lastRowOf(tile) == BM - 1 && nLast == BN - 1) store(acc, sa, tile, Index<1>());
+    bool plain = true;
+    if constexpr(!MX) {
+      bool ok = mild(scalesOf[wn * 64 + lane]);
+#pragma unroll
+      for(int mi = 0; mi < MI; mi++) ok = mild(sa[mi]) && ok;
+      plain = !anyLane(!ok);
+    }
+    if(plain && lastRowOf(tile) == BM - 1 && nLast == BN - 1) store(acc, sa, tile, Index<1>(), Index<0>());
     else {
-      store(acc, sa, tile, Index<0>());
+      if(plain) store(acc, sa, tile, Index<0>(), Index<0>());
+      else store(acc, sa, tile, Index<0>(), Index<1>());
       waitLoads<0>();
     }
   }
@@ -913,7 +957,7 @@ __global__ __launch_bounds__(512) void linear8FewKernel(Linear8Args g) {
     float x = 0.0f;
 #pragma unroll
     for(int w = 0; w < NW; w++) x += sums[w][c][r];
-    if(!MX) x = x * ((const float*)g.aScales)[m0 + r] * ((const float*)g.wScales)[n0 + c];
+    if(!MX) x = scaledByAny(x, ((const float*)g.aScales)[m0 + r], ((const float*)g.wScales)[n0 + c]);
     if(g.bias != nullptr) x += g.bias[n0 + c];
     ((TO*)g.out)[(m0 + r) * g.outStride + n0 + c] = TR::fromFloat(x);
   }

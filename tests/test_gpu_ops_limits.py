@@ -1,0 +1,44 @@
+"""-m gpu: katago_amd.ops at the ends of what it takes - scales, values, lengths and tensors far from the usual ones - against plain formulas in 64 bits."""
+import pytest
+import torch
+
+import ops_ref as ref
+from katago_amd import ops
+from test_gpu_ops import eight, gen
+from test_ops_limits_emulated import check_linear_any, spread_scales
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_grad():
+    with torch.no_grad():
+        yield
+
+
+@pytest.mark.parametrize("out", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 512), (30, 100, 4096), (64, 64, 272), (70, 64, 512), (361, 1152, 384), (200, 3000, 1184), (1000, 4100, 1152),
+                                   (5000, 4999, 512), (72500, 1152, 384), (71681, 1100, 128)])
+def test_linear8_row_scales_of_any_size(m, n, k, out):
+    """Scales from 2^-120 to 2^120 on both sides: a large one must not carry a sum out of fp32 that the other brings back, in any of the kernels"""
+    g, c = gen(m + n), torch.Generator().manual_seed(m + n)
+    (a, _), (w, _) = eight(m, k, "row", g), eight(n, k, "row", g)
+    for sa, sw in ((spread_scales(m, c), spread_scales(n, c)), (torch.rand(m, generator=c) * 1e35, torch.rand(n, generator=c) * 1e-37)):
+        sa, sw = sa.cuda(), sw.cuda()
+        y = ops.linear8(a, sa, w, sw, out_dtype=ref.TYPES[out])
+        for lo in range(0, m, 10000):
+            part = slice(lo, min(m, lo + 10000))
+            check_linear_any(y[part], *ref.linear(ref.values(a[part], sa[part]), ref.values(w, sw)), k)
+
+
+def test_linear8_scales_of_nothing():
+    """Scales of zero, infinity and NaN give what the formula gives, beside rows that are as they always are"""
+    g = gen(2)
+    for m in (5, 70):
+        (a, sa), (w, sw) = eight(m, 256, "row", g), eight(65, 256, "row", g)
+        want = ops.linear8(a, sa, w, sw, out_dtype=torch.float32)
+        sb = sa.clone()
+        sb[1], sb[2], sb[3] = 0.0, float("inf"), float("nan")
+        y = ops.linear8(a, sb, w, sw, out_dtype=torch.float32)
+        assert bool((y[1] == 0).all()) and bool(torch.isinf(y[2]).all()) and bool(torch.isnan(y[3]).all())
+        assert bool(((y - want)[[0, 4]].abs() <= 2 * ref.U * want[[0, 4]].abs()).all())
