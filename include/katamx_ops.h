@@ -41,8 +41,8 @@ enum { KMX_SCALES_NONE = 0, KMX_SCALES_ROW = 1, KMX_SCALES_MX = 2 };
  *   codes, scales = y in e4m3 (of y before its own rounding to `type`)
  * x, residual, sum, y: [rows][channels]; residual and sum are both given or both NULL. weight, beta: float[channels] or NULL (1 and 0);
  * mask: float[rows] or NULL. y and codes may be NULL, not both; codes and scales are NULL with KMX_SCALES_NONE. sum and y may each be the very
- * tensor x or residual (same pointer and stride); no other output may overlap anything. The mean is taken in fp32: a row whose squares
- * overflow it (beyond 1.8e19) is normalised to 0. */
+ * tensor x or residual (same pointer and stride); no other output may overlap anything. The mean is good for all
+ * finite values of the type, those whose squares leave fp32 included; a row of zeros with epsilon 0 is 0 / 0, NaN. */
 typedef struct kmx_rmsnorm_args {
   int32_t type, scale_kind;
   int64_t rows;

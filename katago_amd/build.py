@@ -17,7 +17,7 @@ OBJDIR = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libkatamx.so")
 
 SOURCES = ["conv_mfma.hip", "conv_chain.hip", "pointwise.hip", "conv_bench.hip", "conv_f32.hip", "misc_kernels.hip", "transformer_kernels.hip", "norm_quant.hip", "linear8.hip", "rotary.hip", "engine.cpp", "model_desc.cpp", "kmx_api.cpp", "batcher.cpp", "numa.cpp", "ops_api.cpp"]
-HEADERS = ["kernels.h", "device_common.h", "conv_kernel.h", "conv_chain_kernel.h", "conv_small_kernel.h", "pointwise_kernel.h", "pointwise2_kernel.h", "pointwise3_kernel.h", "engine.h", "model_desc.h", "katamx_tuning.h", "numa.h", "ops.h", os.path.join("..", "..", "include", "katamx.h"), os.path.join("..", "..", "include", "katamx_ops.h")]
+HEADERS = ["kernels.h", "device_common.h", "conv_kernel.h", "conv_chain_kernel.h", "conv_small_kernel.h", "pointwise_kernel.h", "pointwise2_kernel.h", "pointwise3_kernel.h", "engine.h", "model_desc.h", "katamx_tuning.h", "numa.h", "ops.h", "ops_device.h", os.path.join("..", "..", "include", "katamx.h"), os.path.join("..", "..", "include", "katamx_ops.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -fno-slp-vectorize: left on, the SLP vectoriser packs adjacent fp32 epilogue arithmetic into v_pk_*_f32 instructions - which
 # issue no faster than two plain ones on gfx950 and cost ~1.6 v_mov_b64 per value to marshal operands into aligned register

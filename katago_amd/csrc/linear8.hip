@@ -15,8 +15,8 @@
 // bound by the weights' way in: 1 x 4096 x 4096 5.1 us (3.3 TB/s).
 #include <atomic>
 
-#include "device_common.h"
 #include "ops.h"
+#include "ops_device.h"
 
 namespace kmx {
 
@@ -48,14 +48,6 @@ inline void waveBarrier() { __syncthreads(); }
 inline int anew(int x) { return x; }
 inline void countedStore() { emu::vmNote(); }
 template <class V> inline void computed(V&) {}
-inline bool anyLane(bool x) {
-  float v = x ? 1.0f : 0.0f;
-  for(int o = 1; o < 64; o <<= 1) {
-    const float u = __shfl_xor(v, o);
-    v = u > v ? u : v;
-  }
-  return v != 0.0f;
-}
 inline hipError_t computeUnits(int, int* n) {
   *n = 8;  // (few: work-groups go round more than once)
   return hipSuccess;
@@ -91,7 +83,6 @@ __device__ __forceinline__ void computed(V& v) {
 }
 // A store instruction that a later wait's count includes (the emulation enters it into the wave's queue)
 __device__ __forceinline__ void countedStore() {}
-__device__ __forceinline__ bool anyLane(bool x) { return __builtin_amdgcn_ballot_w64(x) != 0; }
 // x, as far as the compiler can tell a new value each time: what is computed from it is not kept in registers around a loop
 __device__ __forceinline__ int anew(int x) {
   asm volatile("" : "+v"(x));

@@ -6,13 +6,13 @@
 //   SCALES_ROW  s = max(max_c |y_c| / 448, 2^-126), 1 where y is all 0;                  code_c = e4m3(y_c / s)
 //   SCALES_MX   s = 2^k with the smallest k >= -127 for which max |y| / s <= 448 over 32 channels, 1 where they are all 0
 //   A row (a block of 32) that holds an infinity or a NaN gets the scale NaN and codes 0.
-// Everything between the loads and the stores is fp32. e4m3 rounds to nearest even: 448 is its largest value, nothing clips.
+// Everything between the loads and the stores is fp32; the sum of squares is fp64 where fp32's is not good enough. e4m3 rounds to nearest even: 448 is its largest value, nothing clips.
 //
 // Bound by memory: a row's values stay in registers, so that everything is read once and written once. 92416 rows of 384 channels in fp16 with residual,
 // mask and codes 51 us (4.9 TB/s; a large copy reaches 5.1), 8190 of 4096 in bf16 with sum, y and codes for 32 channels each 56 us (5.4), the
 // 8-bit form alone of 16383 x 1536 15.6 us (4.9). A few rows are bound by one trip to memory and a launch: 361 x 384 3.3 us.
-#include "device_common.h"
 #include "ops.h"
+#include "ops_device.h"
 
 namespace kmx {
 
@@ -132,14 +132,19 @@ __device__ __forceinline__ void zeroIf(bool spoilt, float (&v)[8]) {
 
 // Sum / largest over the TPR threads of a row; up to a wave through lane exchanges, beyond it through LDS. The order is fixed: the same
 // inputs give the same bits.
-template <int TPR>
-__device__ __forceinline__ float rowSum(float v, float* part) {
+__device__ __forceinline__ float laneXor(float v, int mask) { return __shfl_xor(v, mask); }
+__device__ __forceinline__ double laneXor(double v, int mask) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)shflXorBits((unsigned)(b >> 32), mask) << 32 | shflXorBits((unsigned)b, mask));
+}
+template <int TPR, class S>
+__device__ __forceinline__ S rowSum(S v, S* part) {
 #pragma unroll
-  for(int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += __shfl_xor(v, o);
+  for(int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += laneXor(v, o);
   if constexpr(TPR > 64) {
     if((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = 0.0f;
+    v = 0;
 #pragma unroll
     for(int w = 0; w < TPR / 64; w++) v += part[w];
   }
@@ -162,16 +167,34 @@ __device__ __forceinline__ unsigned rowMax(unsigned v, unsigned* part) {
   return v;
 }
 
-// 1 / sqrt(sum / C + eps) in two parts: fp32's own error in it (up to 2^-23) would be the row's in every channel and move codes and scales that lie next
-// to a border. One Newton step on what is left of 1 - x r^2; a sum that overflowed gives 0, a row of zeros without eps infinity, both without a second part.
+__device__ __forceinline__ void addSquares(double& ss, const float (&v)[8]) {
+#pragma unroll
+  for(int j = 0; j < 8; j++) ss = __builtin_fma((double)v[j], (double)v[j], ss);
+}
+// The mean of the squares + eps. fp32's sum of squares is good while that is within these bounds: below 2^-96 squares lose bits among the subnormals, above 2^126
+// their sum overflows (a NaN is outside).
+__device__ __forceinline__ double meanOf(const NormQuantArgs& a, double sum) { return sum * a.perChannel + (double)a.eps; }
+__device__ __forceinline__ bool ordinary(double mean) { return mean >= 0x1p-96 && mean <= 0x1p126; }
+// mean^(-1/2) in two parts: fp32's own error in it (up to 2^-23) would be the row's in every channel and move codes and scales that lie next to a border.
+// One Newton step on what is left of 1 - x r^2. Where the root or its second part would leave fp32, the row's values are multiplied with `pre` first: 2^100
+// for means below 2^-96 (a subnormal value is then at least 2^-49), 2^-64 above 2^126 (what loses bits by it is below 2^-125 in the result). A row of zeros
+// without eps gives infinity, one with an infinity 0, both without a second part.
 struct Factor {
-  float hi, lo;
+  float hi, lo, pre;
 };
-__device__ __forceinline__ Factor factorOf(const NormQuantArgs& a, float sum) {
-  const double x = (double)sum * a.perChannel + (double)a.eps;
+__device__ __forceinline__ Factor factorOf(double x) {
+  float pre = 1.0f;
+  if(x < 0x1p-96) {
+    x *= 0x1p200;
+    pre = 0x1p100f;
+  }
+  if(x > 0x1p126) {
+    x *= 0x1p-128;
+    pre = 0x1p-64f;
+  }
   const float xh = (float)x, xl = (float)(x - (double)xh), r = rsqrtf(xh);
   const float t = xh * r, left = __builtin_fmaf(-t, r, 1.0f) - (__builtin_fmaf(xh, r, -t) + xl * r) * r, lo = 0.5f * r * left;
-  return Factor{r, __builtin_fabsf(lo) < r * 1e-3f ? lo : 0.0f};
+  return Factor{r, __builtin_fabsf(lo) < r * 1e-3f ? lo : 0.0f, pre};
 }
 // The norm's factor applied to 8 values: v * r * w, rounded once, + beta; 0 on a masked row. (Of 33.5 million codes 8 lie on the other side of a border than
 // the formula's in 64 bits; 15 with fp32's root and each product rounded. 256 boards take 1.3 us longer for it.)
@@ -179,6 +202,10 @@ __device__ __forceinline__ void scale8(const NormQuantArgs& a, int c, Factor r, 
   if(!a.normed) return;
   float w[8];
   if(a.weight != nullptr) load8<TraitsF32>(a.weight, c, a.C, w);
+  if(__builtin_expect(r.pre != 1.0f, 0)) {
+#pragma unroll
+    for(int i = 0; i < 8; i++) v[i] *= r.pre;
+  }
 #pragma unroll
   for(int i = 0; i < 8; i++) {
     const float p = v[i] * r.hi, e = __builtin_fmaf(v[i], r.lo, __builtin_fmaf(v[i], r.hi, -p));
@@ -220,11 +247,12 @@ __device__ __forceinline__ void mx8(const NormQuantArgs& a, int64_t row, int c, 
 }
 
 // A row on TPR threads, its values in registers: 8 consecutive channels a thread and round, NCH rounds. x and residual are read once, everything
-// else is written once.
+// else is written once. (Of 1024 threads a CU holds two work-groups, if a thread has 64 registers; fp32 has 80 at four pieces.)
 template <class TR, int TPR, int NCH>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void normQuantKernel(NormQuantArgs a) {
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR == 1024 && sizeof(typename TR::T) == 2 ? 8 : 1) void normQuantKernel(NormQuantArgs a) {
   constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
   __shared__ float part[2][TPR > 64 ? TPR / 64 : 1];
+  __shared__ double partWide[TPR > 64 ? TPR / 64 : 1];
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const bool valid = row < a.rows;  // (lanes without a row stay for the exchanges)
@@ -238,8 +266,18 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void normQuantKernel(NormQua
 #pragma unroll
     for(int j = 0; j < 8; j++) ss += v[i][j] * v[i][j];
   }
-  Factor r = {1.0f, 0.0f};
-  if(a.normed) r = factorOf(a, rowSum<TPR>(ss, part[0]));
+  Factor r = {1.0f, 0.0f, 1.0f};
+  if(a.normed) {
+    double mean = meanOf(a, rowSum<TPR>(ss, part[0]));
+    if(__builtin_expect(anyLane(!ordinary(mean)), 0)) {  // such rows again in fp64 (for every row 92416 of 384 channels take 4.6 us longer)
+      double wide = 0.0;
+#pragma unroll
+      for(int i = 0; i < NCH; i++) addSquares(wide, v[i]);
+      wide = rowSum<TPR>(wide, partWide);  // (rows of more than a wave: one to a work-group, all of it is here)
+      if(!ordinary(mean)) mean = meanOf(a, wide);
+    }
+    r = factorOf(mean);
+  }
   const bool on = a.mask == nullptr || !valid || a.mask[row] != 0.0f;
   unsigned top = 0;
 #pragma unroll
@@ -282,19 +320,19 @@ template <class TR>
 __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
   typedef typename TR::T T;
   constexpr int TPR = 1024;
-  __shared__ float part[2][TPR / 64];
+  __shared__ double part[TPR / 64];
+  __shared__ unsigned partTop[TPR / 64];
   const int64_t row = blockIdx.x;
   const T* const h = a.residual != nullptr ? (const T*)a.sum + row * a.sumStride : (const T*)a.x + row * a.xStride;
   float v[8];
-  Factor r = {1.0f, 0.0f};
+  Factor r = {1.0f, 0.0f, 1.0f};
   if(a.normed) {
-    float ss = 0.0f;
+    double ss = 0.0;  // (a lane's terms are many: in fp32 2^24 channels of one value are 920 roundings off)
     for(int c = threadIdx.x * 8; c < a.C; c += TPR * 8) {
       stream8<TR, false>(a, row, c, v);
-#pragma unroll
-      for(int j = 0; j < 8; j++) ss += v[j] * v[j];
+      addSquares(ss, v);
     }
-    r = factorOf(a, rowSum<TPR>(ss, part[0]));
+    r = factorOf(meanOf(a, rowSum<TPR>(ss, part)));
   }
   const bool on = a.mask == nullptr || a.mask[row] != 0.0f;
   float scale = 1.0f, inv = 1.0f;
@@ -306,7 +344,7 @@ __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
       const unsigned m = maxBits(v);
       top = m > top ? m : top;
     }
-    rowScale(rowMax<TPR>(top, (unsigned*)part[1]), scale, inv);
+    rowScale(rowMax<TPR>(top, partTop), scale, inv);
     if(threadIdx.x == 0) ((float*)a.scales)[row] = scale;
   }
   for(int c0 = 0; c0 < a.C; c0 += TPR * 8) {  // (all lanes take part in a block's exchanges)

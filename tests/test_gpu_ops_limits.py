@@ -5,7 +5,7 @@ import torch
 import ops_ref as ref
 from katago_amd import ops
 from test_gpu_ops import eight, gen
-from test_ops_limits_emulated import check_linear_any, spread_scales
+from test_ops_limits_emulated import check_linear_any, rows_of_any_size, spread_scales
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,29 @@ def test_linear8_scales_of_nothing():
         y = ops.linear8(a, sb, w, sw, out_dtype=torch.float32)
         assert bool((y[1] == 0).all()) and bool(torch.isinf(y[2]).all()) and bool(torch.isnan(y[3]).all())
         assert bool(((y - want)[[0, 4]].abs() <= 2 * ref.U * want[[0, 4]].abs()).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("c", [50, 96, 384, 1000, 2000, 4096, 8000, 20000, 33000])
+def test_rms_norm_of_small_and_large_rows(c, dtype):
+    """Without eps: the squares of values below 1e-19 or beyond 1.8e19 leave fp32, their rows' norms are ordinary numbers; on lanes for few rows and for many"""
+    x = rows_of_any_size(c, ref.TYPES[dtype], torch.Generator().manual_seed(c)).cuda()
+    for again in (1, 300):
+        many = x.repeat(again, 1)
+        n = ops.rms_norm(many, eps=0.0, scales="row", want_y=True)
+        some = many.abs().amax(1) > 0
+        want = ref.norm(many[some], eps=0.0)[1]
+        ref.check_y(n.y[some], want)
+        ref.check_codes(n.codes[some], n.scales[some], want, ref.norm_slack(want))
+        assert bool(torch.isnan(n.y[~some]).all()) and bool(torch.isnan(n.scales[~some]).all())
+        for row in range(0, x.shape[0], 5):
+            alone = ops.rms_norm(many[row:row + 1], eps=0.0).y[0]
+            if again == 1:
+                assert torch.equal(alone.nan_to_num(7.0), n.y[row].nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("c", [1 << 22, (1 << 26) + 3])
+def test_rms_norm_of_a_very_long_row(c):
+    """One value in all channels: thousands of squares a lane, whose sum must not collect a rounding each"""
+    x = torch.full((1, c), 1.1, device="cuda")
+    ref.check_y(ops.rms_norm(x, eps=0.0).y, ref.norm(x, eps=0.0)[1])

@@ -56,3 +56,48 @@ def test_linear8_row_scales_of_any_size(emu, m, n, k, out):  # noqa: F811
     # one side all large, the other all small: every result is an ordinary number
     sa, sw = torch.rand(m, generator=g) * 1e35, torch.rand(n, generator=g) * 1e-37
     check_linear_any(linear(emu, a, sa, w, sw, out, 1), *ref.linear(ref.values(a, sa), ref.values(w, sw)), k)
+
+
+def rows_of_any_size(c, t, gen):
+    """rows whose values are normal ones times a power of two each, from the type's smallest number to its largest, ordinary rows between them"""
+    low, high = {torch.float16: (-22, 13), torch.bfloat16: (-131, 125), torch.float32: (-147, 125)}[t]
+    e = list(range(low, high, 23 if t != torch.float16 else 5)) + [-51, -47, 62, 64, high] * (t != torch.float16)
+    e = [v for x in e for v in (x, 0)]
+    x = torch.randn(len(e), c, generator=gen, dtype=torch.float64).clamp(-3.9, 3.9)
+    return (x * torch.exp2(torch.tensor(e).double())[:, None]).to(t)
+
+
+@pytest.mark.parametrize("c", [50, 96, 384, 1000, 5000, 33000])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_rms_norm_of_small_and_large_rows(emu, c, dtype):  # noqa: F811
+    """Without eps: the squares of values below 1e-19 or beyond 1.8e19 leave fp32, their rows' norms are ordinary numbers. A row's result does not depend
+    on what the others of its wave are."""
+    t = ref.TYPES[dtype]
+    x = rows_of_any_size(c, t, torch.Generator().manual_seed(c))
+    n = x.shape[0]
+
+    def call(x):
+        y, codes, sc = torch.zeros_like(x), torch.zeros(x.shape, dtype=torch.float8_e4m3fn), torch.zeros(x.shape[0])
+        a = capi.RmsNormArgs(type=PREC[dtype], scale_kind=1, rows=x.shape[0], channels=c, epsilon=0.0, x=x.data_ptr(), y=y.data_ptr(), codes=codes.data_ptr(),
+                             scales=sc.data_ptr(), x_stride=c, y_stride=c, codes_stride=c)
+        ok(emu, emu.kmx_rmsnorm(0, None, ctypes.byref(a)))
+        return y, codes, sc
+
+    y, codes, sc = call(x)
+    some = x.abs().amax(1) > 0  # (16 bits: a row of the smallest numbers may be all zeros)
+    want = ref.norm(x[some], eps=0.0)[1]
+    ref.check_y(y[some], want)
+    ref.check_codes(codes[some], sc[some], want, ref.norm_slack(want))
+    assert bool(torch.isnan(y[~some].float()).all())  # 0 / 0
+    for row in range(0, n, 7):
+        assert torch.equal(call(x[row:row + 1].clone())[0][0].float().nan_to_num(7.0), y[row].float().nan_to_num(7.0))
+
+
+def test_rms_norm_of_a_very_long_row(emu):  # noqa: F811
+    """4 million channels of one value: 4096 squares a lane, whose sum must not collect a rounding each"""
+    c = (1 << 22) + 8
+    x = torch.full((1, c), 1.1)
+    y = torch.zeros_like(x)
+    a = capi.RmsNormArgs(type=capi.PREC_FP32, rows=1, channels=c, epsilon=0.0, x=x.data_ptr(), y=y.data_ptr(), x_stride=c, y_stride=c)
+    ok(emu, emu.kmx_rmsnorm(0, None, ctypes.byref(a)))
+    ref.check_y(y, ref.norm(x, eps=0.0)[1])
