@@ -6,7 +6,7 @@
 //   SCALES_ROW  s = max(max_c |y_c| / 448, 2^-126), 1 where y is all 0;                  code_c = e4m3(y_c / s)
 //   SCALES_MX   s = 2^k with the smallest k >= -127 for which max |y| / s <= 448 over 32 channels, 1 where they are all 0
 //   A row (a block of 32) that holds an infinity or a NaN gets the scale NaN and codes 0.
-// Everything between the loads and the stores is fp32; the sum of squares is fp64 where fp32's is not good enough. e4m3 rounds to nearest even: 448 is its largest value, nothing clips.
+// Everything between the loads and the stores is fp32; the sum of squares is fp64 where fp32's is not good enough. e4m3 rounds to nearest even.
 //
 // Bound by memory: a row's values stay in registers, so that everything is read once and written once. 92416 rows of 384 channels in fp16 with residual,
 // mask and codes 51 us (4.9 TB/s; a large copy reaches 5.1), 8190 of 4096 in bf16 with sum, y and codes for 32 channels each 56 us (5.4), the
@@ -60,10 +60,23 @@ __device__ __forceinline__ void store8(typename TR::T* p, int c, int C, const fl
       if(c + i < C) p[c + i] = TR::fromFloat(v[i]);
   }
 }
-__device__ __forceinline__ void storeCodes8(uint8_t* p, int c, int C, const float (&v)[8], float inv) {
+// What a row's or a block's values are divided by. inv = 1 / scale, rounded; of a power of two (EXACT) it is exact. Otherwise the product with it would be off
+// by up to two roundings and put values at the border of two codes on the other side (11871 of 25.2 million bf16 values, 1686 of fp16); a step on what it leaves makes
+// it the rounded quotient.
+struct Divisor {
+  float scale, inv;
+};
+template <bool EXACT>
+__device__ __forceinline__ float dividedBy(float v, Divisor d) {
+  const float q = v * d.inv;
+  return EXACT ? q : __builtin_fmaf(__builtin_fmaf(-q, d.scale, v), d.inv, q);
+}
+// (a quotient may lie a rounding beyond 448)
+template <bool EXACT>
+__device__ __forceinline__ void storeCodes8(uint8_t* p, int c, int C, const float (&v)[8], Divisor d) {
   float u[8];
 #pragma unroll
-  for(int i = 0; i < 8; i++) u[i] = __builtin_fminf(__builtin_fmaxf(v[i] * inv, -E4M3_MAX), E4M3_MAX);
+  for(int i = 0; i < 8; i++) u[i] = __builtin_fminf(__builtin_fmaxf(dividedBy<EXACT>(v[i], d), -E4M3_MAX), E4M3_MAX);
   int lo = 0, hi = 0;
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], lo, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], lo, true);
@@ -94,18 +107,16 @@ __device__ __forceinline__ unsigned maxBits(const float (&v)[8]) {
 }
 __device__ __forceinline__ unsigned shflXorBits(unsigned v, int mask) { return bitsOf(__shfl_xor(floatOf(v), mask)); }
 
-// The row's scale and what its values are multiplied with, from the bits of its largest magnitude
-__device__ __forceinline__ void rowScale(unsigned top, float& scale, float& inv) {
-  if(top >= 0x7f800000u) {
-    scale = floatOf(0x7fc00000u);
-    inv = 0.0f;
-  }
-  else if(top == 0) scale = inv = 1.0f;
-  else {
+// The row's scale and what its values are divided by, from the bits of its largest magnitude (a spoilt row's values are zeros by then: by 1)
+__device__ __forceinline__ bool spoilt(unsigned top) { return top >= 0x7f800000u; }
+__device__ __forceinline__ void rowScale(unsigned top, float& scale, Divisor& d) {
+  scale = 1.0f;
+  if(!spoilt(top) && top != 0) {
     scale = floatOf(top) / E4M3_MAX;
     if(scale < 1.17549435e-38f) scale = 1.17549435e-38f;
-    inv = 1.0f / scale;
   }
+  d = Divisor{scale, 1.0f / scale};
+  if(spoilt(top)) scale = floatOf(0x7fc00000u);
 }
 // ... and a block's e8m0 code: top = (1 + m) 2^(e - 127), 448 = 1.75 * 2^8, so k = e - 127 - 8, one more where 1 + m > 1.75
 __device__ __forceinline__ void mxScale(unsigned top, unsigned& code, float& inv) {
@@ -238,11 +249,11 @@ __device__ __forceinline__ void mx8(const NormQuantArgs& a, int64_t row, int c, 
   u = shflXorBits(top, 2);
   top = u > top ? u : top;
   unsigned code;
-  float inv;
-  mxScale(top, code, inv);
+  Divisor d = {1.0f, 1.0f};
+  mxScale(top, code, d.inv);
   zeroIf(code == 255, v);
   if(!in) return;
-  storeCodes8(a.codes + row * a.codesStride, c, a.C, v, inv);
+  storeCodes8<true>(a.codes + row * a.codesStride, c, a.C, v, d);
   if((c & (MX_BLOCK - 1)) == 0) ((uint8_t*)a.scales)[row * (a.C / MX_BLOCK) + c / MX_BLOCK] = (uint8_t)code;
 }
 
@@ -294,14 +305,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR == 1024 && sizeof(typena
   }
   if(a.scaleKind == SCALES_ROW) {
     top = rowMax<TPR>(top, (unsigned*)part[1]);
-    float scale, inv;
-    rowScale(top, scale, inv);
+    float scale;
+    Divisor d;
+    rowScale(top, scale, d);
 #pragma unroll
     for(int i = 0; i < NCH; i++) {
       const int c = (t + i * TPR) * 8;
       if(!valid || c >= a.C) continue;
-      zeroIf(inv == 0.0f, v[i]);
-      storeCodes8(a.codes + row * a.codesStride, c, a.C, v[i], inv);
+      zeroIf(spoilt(top), v[i]);
+      storeCodes8<false>(a.codes + row * a.codesStride, c, a.C, v[i], d);
     }
     if(valid && t == 0) ((float*)a.scales)[row] = scale;
   }
@@ -335,16 +347,18 @@ __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
     r = factorOf(meanOf(a, rowSum<TPR>(ss, part)));
   }
   const bool on = a.mask == nullptr || a.mask[row] != 0.0f;
-  float scale = 1.0f, inv = 1.0f;
+  Divisor d = {1.0f, 1.0f};
+  unsigned top = 0;
   if(a.scaleKind == SCALES_ROW) {
-    unsigned top = 0;
     for(int c = threadIdx.x * 8; c < a.C; c += TPR * 8) {
       load8<TR>(h, c, a.C, v);
       scale8(a, c, r, on, v);
       const unsigned m = maxBits(v);
       top = m > top ? m : top;
     }
-    rowScale(rowMax<TPR>(top, partTop), scale, inv);
+    top = rowMax<TPR>(top, partTop);
+    float scale;
+    rowScale(top, scale, d);
     if(threadIdx.x == 0) ((float*)a.scales)[row] = scale;
   }
   for(int c0 = 0; c0 < a.C; c0 += TPR * 8) {  // (all lanes take part in a block's exchanges)
@@ -357,8 +371,8 @@ __global__ __launch_bounds__(1024) void normQuantLongKernel(NormQuantArgs a) {
       if(a.y != nullptr) store8<TR>((T*)a.y + row * a.yStride, c, a.C, v);
     }
     if(a.scaleKind == SCALES_ROW && in) {
-      zeroIf(inv == 0.0f, v);
-      storeCodes8(a.codes + row * a.codesStride, c, a.C, v, inv);
+      zeroIf(spoilt(top), v);
+      storeCodes8<false>(a.codes + row * a.codesStride, c, a.C, v, d);
     }
     else if(a.scaleKind == SCALES_MX) mx8(a, row, c, in, v);
   }

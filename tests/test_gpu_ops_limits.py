@@ -5,7 +5,7 @@ import torch
 import ops_ref as ref
 from katago_amd import ops
 from test_gpu_ops import eight, gen
-from test_ops_limits_emulated import check_linear_any, rows_of_any_size, spread_scales
+from test_ops_limits_emulated import check_linear_any, rounded_quotients, rows_of_any_size, spread_scales
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,18 @@ def test_rms_norm_of_a_very_long_row(c):
     """One value in all channels: thousands of squares a lane, whose sum must not collect a rounding each"""
     x = torch.full((1, c), 1.1, device="cuda")
     ref.check_y(ops.rms_norm(x, eps=0.0).y, ref.norm(x, eps=0.0)[1])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_codes_are_rounded_quotients(dtype):
+    """16-bit values lie on the border of two codes often enough that a product with the rounded reciprocal is told from the quotient; what a norm
+    codes is its fp32 result"""
+    g, t = gen(3), ref.TYPES[dtype]
+    for rows, c in ((16383, 1536), (361, 384), (5, 8190), (3, 70000)):
+        x = (torch.randn(rows, c, device="cuda", generator=g) * 3).to(t)
+        codes, s = ops.quantize(x)
+        assert torch.equal(s, (x.abs().amax(1).double() / 448).float())  # (torch multiplies a device tensor with 1 / 448)
+        assert torch.equal(codes.view(torch.uint8), rounded_quotients(x, s))
+        if dtype == "fp32":
+            n = ops.rms_norm(x, scales="row", want_y=True)
+            assert torch.equal(n.codes.view(torch.uint8), rounded_quotients(n.y, n.scales))
