@@ -5,7 +5,7 @@ import torch
 import ops_ref as ref
 from katago_amd import ops
 from test_gpu_ops import eight, gen
-from test_ops_limits_emulated import check_linear_any, rounded_quotients, rows_of_any_size, spread_scales
+from test_ops_limits_emulated import check_linear_any, check_small_results, rounded_quotients, rows_of_any_size, small_sine_angles, spread_scales
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,19 @@ def test_codes_are_rounded_quotients(dtype):
         if dtype == "fp32":
             n = ops.rms_norm(x, scales="row", want_y=True)
             assert torch.equal(n.codes.view(torch.uint8), rounded_quotients(n.y, n.scales))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_of_small_sines(layout):
+    """A sine next to 0 or to pi, a cosine next to pi / 2, in fp32: right relative to itself"""
+    angle = small_sine_angles().cuda()
+    n = angle.shape[0]
+    for pairs in (1, 4, 8):  # pieces of one pair and of four
+        q = torch.eye(2, device="cuda").repeat(n, 1).reshape(1, 2 * n, 2, 1).expand(1, 2 * n, 2, pairs)
+        q = (q if layout == "half" else q.transpose(2, 3)).reshape(1, 2 * n, 2 * pairs).contiguous()
+        f = angle.reshape(n, 1, 1).expand(n, 1, pairs).contiguous()
+        for magnitude in (1.0, 1.375):
+            y = ops.rotary(q, None, torch.ones(1, device="cuda", dtype=torch.int32), f, layout=layout, magnitude=magnitude)[0]
+            y = y.reshape(n, 2, 2, pairs) if layout == "half" else y.reshape(n, 2, pairs, 2).transpose(2, 3)
+            for p in range(pairs):
+                check_small_results(y[..., p], angle, magnitude)

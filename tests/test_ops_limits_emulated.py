@@ -7,7 +7,7 @@ import torch
 
 import ops_ref as ref
 from katago_amd import capi
-from test_ops_emulated import PREC, Guarded, aligned_copy, eight, emu, ok  # noqa: F401 (emu: the fixture)
+from test_ops_emulated import PREC, Guarded, aligned_copy, eight, emu, ok, rotary_args  # noqa: F401 (emu: the fixture)
 
 
 def check_linear_any(got, want, mag, k):
@@ -118,3 +118,32 @@ def test_quantize_divides(emu, dtype):  # noqa: F811
         ok(emu, emu.kmx_quantize(0, None, PREC[dtype], 1, rows, c, x.data_ptr(), c, codes.data_ptr(), c, sc.data_ptr()))
         assert torch.equal(sc, x.float().abs().amax(1) / 448)
         assert torch.equal(codes, rounded_quotients(x, sc))
+
+
+def small_sine_angles():
+    """angles next to 0 and to quarters and halves of a turn, to either side, and between these"""
+    near = torch.exp2(-torch.arange(2, 40, 0.25).double())
+    places = torch.arange(-4, 5).double() / 4
+    turns = (places[:, None, None] + torch.stack([near, -near])[None]).reshape(-1)
+    return turns * 2 * torch.pi
+
+
+def check_small_results(got, angle, magnitude=1.0):
+    """(0, 1) and (1, 0) turned by `angle`: the results are the sine and the cosine themselves, each to be right relative to itself. fp32's roundings on the
+    way: the reduced angle, three of the series' last steps, the magnitude, the result: 6 U, and 2 U for the steps before; the angle in turns
+    is an fp64 number, off by 2^-53 of its size three times."""
+    sin, cos = angle.sin() * magnitude, angle.cos() * magnitude
+    for g, w in ((got[:, 0, 0], cos), (got[:, 0, 1], sin), (got[:, 1, 0], -sin), (got[:, 1, 1], cos)):
+        far = (g.double() - w).abs()
+        bound = 8 * ref.U * w.abs() + magnitude * 2.0 ** -50 * angle.abs()
+        assert bool((far <= bound).all()), float((far / bound).max())
+
+
+def test_rotary_of_small_sines(emu):  # noqa: F811
+    """A sine next to 0 or to pi, a cosine next to pi / 2, in fp32"""
+    angle = small_sine_angles()
+    n = angle.shape[0]
+    q = torch.eye(2).repeat(n, 1).reshape(1, 1, 2 * n, 2)  # two heads for each frequency
+    out, pos, f = torch.empty_like(q), torch.ones(1, 1, 1, dtype=torch.int32), angle.reshape(n, 1, 1)
+    ok(emu, emu.kmx_rotary(0, None, ctypes.byref(rotary_args(q, None, out, None, pos, f, "fp32", False, 1.0, False))))
+    check_small_results(out.reshape(n, 2, 2), angle)
