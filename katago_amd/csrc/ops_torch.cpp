@@ -51,10 +51,13 @@ Arg tensor(const char* name, PyObject* o) {
   if(!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
   return Arg{name, THPVariable_Unpack(o)};
 }
-// The index of the device all of them are on; gradients are refused
+// The index of the device all of them are on; gradients are refused, forward-mode tangents too (that mode is on in no_grad as well)
 int onDevice(std::initializer_list<const Arg*> args) {
   int index = -1;
   const bool grad = c10::GradMode::is_enabled();
+  for(const Arg* a : args)
+    if(a->given() && a->t._fw_grad(0).defined())
+      refuse(std::string(a->name) + " carries a forward-mode tangent and the operators compute none: unpack it first");
   for(const Arg* a : args) {
     if(!a->given()) continue;
     const c10::Device d = a->t.device();

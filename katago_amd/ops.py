@@ -8,7 +8,8 @@
 
 Each call runs on the current stream of its tensors' device, returns without waiting, allocates nothing but the outputs it returns, and gives the
 same bits for the same inputs; it may be captured into a graph. Bad arguments raise KatamxError before anything is launched. The operators
-compute no gradients: a tensor that requires one is refused outside torch.no_grad() (rotary(inverse=True) is the transpose of rotary()).
+compute no gradients: a tensor that requires one is refused outside torch.no_grad(), one with a forward-mode tangent everywhere (rotary(inverse=True) is the
+transpose of rotary()).
 """
 import collections
 import ctypes

@@ -1,9 +1,11 @@
 """-m gpu: katago_amd.ops at the ends of what it takes - scales, values, lengths and tensors far from the usual ones - against plain formulas in 64 bits."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import ops_ref as ref
 from katago_amd import ops
+from katago_amd.capi import KatamxError
 from test_gpu_ops import eight, gen
 from test_ops_limits_emulated import check_linear_any, check_small_results, rounded_quotients, rows_of_any_size, small_sine_angles, spread_scales
 
@@ -99,3 +101,21 @@ def test_rotary_of_small_sines(layout):
             y = y.reshape(n, 2, 2, pairs) if layout == "half" else y.reshape(n, 2, pairs, 2).transpose(2, 3)
             for p in range(pairs):
                 check_small_results(y[..., p], angle, magnitude)
+
+
+def test_forward_mode_tangents_are_refused():
+    x, f, pos = torch.ones(4, 2, 32, device="cuda"), torch.ones(16, device="cuda").double(), torch.zeros(4, device="cuda", dtype=torch.int32)
+    w, (codes, s) = torch.ones(32, device="cuda"), ops.quantize(torch.ones(4, 32, device="cuda"))
+    ones = torch.ones(4, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.rms_norm(dual(x)), lambda: ops.rms_norm(x, dual(w)), lambda: ops.rms_norm(x, residual=dual(x)), lambda: ops.rms_norm(x, y_out=dual(x)),
+                     lambda: ops.quantize(dual(x)), lambda: ops.linear8(codes, dual(s), codes, s), lambda: ops.linear8(codes, s, codes, s, dual(ones)),
+                     lambda: ops.rotary(dual(x), None, pos, f), lambda: ops.rotary(x, dual(x), pos, f), lambda: ops.rotary(x, None, pos, dual(f))):
+            with pytest.raises(KatamxError, match="tangent"):
+                call()
+            with torch.enable_grad(), pytest.raises(KatamxError, match="tangent"):
+                call()
+        primal = forward_ad.unpack_dual(dual(x)).primal
+        ops.rms_norm(primal)
