@@ -148,6 +148,11 @@ class WithoutGil {
  private:
   PyThreadState* state_;
 };
+// A tensor of the caller's has been written: autograd, which may keep it for a backward pass, is told as torch's own in-place operations tell it. (Inference
+// tensors have no version.)
+void written(const Arg& a) {
+  if(a.given() && !a.t.is_inference()) a.t.unsafeGetTensorImpl()->bump_version();
+}
 // (the message is of this thread's last call)
 void check(int rc) {
   if(rc != KMX_OK) throw Refused{rc, entry.lastError()};
@@ -228,6 +233,8 @@ PyObject* rmsNorm(PyObject* const* args, Py_ssize_t n) {
       a.codes_stride = r.channels;
     }
     if(r.n > 0) check(entry.rmsnorm(device, stream, &a));
+    written(sumOut);
+    written(yOut);
   }
   return Py_BuildValue("(NNNN)", wrapped(sum.t), wrapped(y.t), wrapped(codes), wrapped(scales));
 }
@@ -305,6 +312,7 @@ PyObject* linear8(PyObject* const* args, Py_ssize_t n) {
     a.out = out->data_ptr();
     a.out_stride = rowsOf(out).stride;
     if(r.n > 0) check(entry.linear8(device, stream, &a));
+    written(given);
   }
   return wrapped(out.t);
 }
@@ -386,6 +394,8 @@ PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
       a.k = side(k, ko);
     }
     if(a.batch > 0 && a.seq > 0) check(entry.rotary(device, stream, &a));
+    written(qOut);
+    written(kOut);
   }
   return Py_BuildValue("(NN)", wrapped(qo.t), wrapped(ko.t));
 }

@@ -119,3 +119,31 @@ def test_forward_mode_tangents_are_refused():
                 call()
         primal = forward_ad.unpack_dual(dual(x)).primal
         ops.rms_norm(primal)
+
+
+def test_written_tensors_have_a_new_version():
+    """A tensor that autograd keeps for a backward pass and an operator writes over is noticed there, as with torch's own in-place operations"""
+    x, pos, f = torch.ones(4, 2, 32, device="cuda"), torch.zeros(4, device="cuda", dtype=torch.int32), torch.ones(16, device="cuda").double()
+    codes, s = ops.quantize(torch.ones(4, 32, device="cuda"))
+    for write in (lambda t: ops.rms_norm(x, y_out=t), lambda t: ops.rms_norm(x, residual=x, sum_out=t), lambda t: ops.rms_norm(t, y_out=t),
+                  lambda t: ops.rotary(x, None, pos, f, q_out=t), lambda t: ops.rotary(x, x, pos, f, k_out=t), lambda t: ops.rotary(t, None, pos, f, q_out=t),
+                  lambda t: ops.linear8(codes, s, codes, s, out=t.reshape(-1)[:16].reshape(4, 4))):
+        with torch.enable_grad():
+            leaf, kept = torch.ones(4, 2, 32, device="cuda", requires_grad=True), torch.ones(4, 2, 32, device="cuda")
+            loss = (leaf * kept).sum()
+        before = kept._version
+        write(kept)
+        assert kept._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = x._version, codes._version
+    ops.rms_norm(x, residual=x, scales="row")
+    ops.rotary(x, x, pos, f)
+    assert (x._version, codes._version) == before  # what is only read
+    with pytest.raises(KatamxError):
+        ops.rms_norm(x, y_out=x[:2])
+    assert x._version == before[0]  # a refused call writes nothing
+    with torch.inference_mode():
+        t = torch.ones(4, 32, device="cuda")
+        ops.rms_norm(t, y_out=t)
+    ops.rms_norm(t, y_out=t)  # (a tensor without a version, outside the mode it was made in)
