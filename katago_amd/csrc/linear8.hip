@@ -956,9 +956,7 @@ __global__ __launch_bounds__(512) void linear8FewKernel(Linear8Args g) {
 
 template <int MT, bool MX, int OUT>
 hipError_t launchFew(const Linear8Args& g, hipStream_t stream) {
-  auto kern = linear8FewKernel<MT, MX, OUT>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((g.N + 15) / 16), (unsigned)((g.rows + 16 * MT - 1) / (16 * MT))), dim3(512), 0, stream, g);
-  return hipGetLastError();
+  return launchKernel(linear8FewKernel<MT, MX, OUT>, dim3((unsigned)((g.N + 15) / 16), (unsigned)((g.rows + 16 * MT - 1) / (16 * MT))), dim3(512), 0, stream, g);
 }
 // The current device's compute units, asked for once per instantiation and device (cus: 0 until then); a kernel's large LDS window is opted in to there
 constexpr int MAX_DEVICES = 64;
@@ -992,8 +990,7 @@ hipError_t launchTile(const Linear8Args& g, hipStream_t stream) {
   const hipError_t e = prepared(kern, LDS, cus, &n);
   if(e != hipSuccess) return e;
   const int64_t most = (int64_t)n * PER_CU / 8 * 8;  // (a multiple of the XCDs: a work-group's tiles stay on its XCD's part)
-  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles < most ? tiles : most)), dim3(64 * WM * WN), LDS, stream, g);
-  return hipGetLastError();
+  return launchKernel(kern, dim3((unsigned)(tiles < most ? tiles : most)), dim3(64 * WM * WN), LDS, stream, g);
 }
 template <int KS, bool MX, int OUT>
 hipError_t launchShort(const Linear8Args& g, int groups, hipStream_t stream) {
@@ -1003,8 +1000,7 @@ hipError_t launchShort(const Linear8Args& g, int groups, hipStream_t stream) {
   int n = 0;
   const hipError_t e = prepared(kern, LDS, cus, &n);
   if(e != hipSuccess) return e;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(8 * groups * ((g.N + 127) / 128))), dim3(256), LDS, stream, g, groups);
-  return hipGetLastError();
+  return launchKernel(kern, dim3((unsigned)(8 * groups * ((g.N + 127) / 128))), dim3(256), LDS, stream, g, groups);
 }
 template <bool MX, int OUT>
 hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {

@@ -400,9 +400,9 @@ hipError_t launchRows(const NormQuantArgs& a, hipStream_t stream) {
   constexpr int64_t MOST = (int64_t)0x7fffffff / BLOCK * RPB;
   for(int64_t first = 0; first < a.rows; first += MOST) {
     const NormQuantArgs b = rowsFrom<TR>(a, first, MOST);
-    if constexpr(NCH > 0) hipLaunchKernelGGL((normQuantKernel<TR, TPR, NCH>), dim3((unsigned)((b.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, stream, b);
-    else hipLaunchKernelGGL(normQuantLongKernel<TR>, dim3((unsigned)b.rows), dim3(BLOCK), 0, stream, b);
-    const hipError_t e = hipGetLastError();
+    hipError_t e;
+    if constexpr(NCH > 0) e = launchKernel(normQuantKernel<TR, TPR, NCH>, dim3((unsigned)((b.rows + RPB - 1) / RPB)), dim3(BLOCK), 0, stream, b);
+    else e = launchKernel(normQuantLongKernel<TR>, dim3((unsigned)b.rows), dim3(BLOCK), 0, stream, b);
     if(e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -2,9 +2,27 @@
 #ifndef KMX_OPS_DEVICE_H_
 #define KMX_OPS_DEVICE_H_
 
+#include <tuple>
+
 #include "device_common.h"
 
 namespace kmx {
+
+// A launch, and ITS error: what an earlier call of the program left for hipGetLastError() stays there, and is not reported as this one's
+template <class... P, class... A>
+hipError_t launchKernel(void (*kern)(P...), dim3 grid, dim3 block, int lds, hipStream_t stream, const A&... args) {
+  static_assert(sizeof...(P) == sizeof...(A), "arguments");
+#ifdef KMX_EMULATED_HIP
+  hipLaunchKernelGGL(kern, grid, block, lds, stream, args...);
+  return hipSuccess;
+#else
+  std::tuple<P...> copies(args...);
+  return std::apply([&](P&... p) {
+    void* at[] = {(void*)&p...};
+    return hipLaunchKernel((const void*)kern, grid, block, at, (size_t)lds, stream);
+  }, copies);
+#endif
+}
 
 // Has any lane of the wave x?
 #ifdef KMX_EMULATED_HIP

@@ -9,8 +9,8 @@
 //
 // Bound by memory: 4 x 8191 tokens of 32 + 8 heads of 128 in bf16 124 us (5.4 TB/s; a large copy reaches 5.1), 256 boards of 12 + 6 heads of 32 in fp16
 // with learned frequencies 49 us (4.4). Eight tokens take 3.0 us, a launch and two trips to memory.
-#include "device_common.h"
 #include "ops.h"
+#include "ops_device.h"
 
 namespace kmx {
 
@@ -198,9 +198,7 @@ hipError_t launchPieces(const RotaryArgs& a, hipStream_t stream) {
     const int64_t n = a.tokens - t0 < most ? a.tokens - t0 : most;
     r.token0 = (unsigned)t0;
     r.threads = (unsigned)(n * perToken);
-    auto kern = rotaryKernel<TR, PV, HALF>;
-    hipLaunchKernelGGL(kern, dim3((r.threads + 255) / 256), dim3(256), 0, stream, r);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = launchKernel(rotaryKernel<TR, PV, HALF>, dim3((r.threads + 255) / 256), dim3(256), 0, stream, r);
     if(e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -1,10 +1,12 @@
 """-m gpu: katago_amd.ops at the ends of what it takes - scales, values, lengths and tensors far from the usual ones - against plain formulas in 64 bits."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import ops_ref as ref
-from katago_amd import ops
+from katago_amd import capi, ops
 from katago_amd.capi import KatamxError
 from test_gpu_ops import eight, gen
 from test_ops_limits_emulated import check_linear_any, check_small_results, rounded_quotients, rows_of_any_size, small_sine_angles, spread_scales
@@ -147,3 +149,29 @@ def test_written_tensors_have_a_new_version():
         t = torch.ones(4, 32, device="cuda")
         ops.rms_norm(t, y_out=t)
     ops.rms_norm(t, y_out=t)  # (a tensor without a version, outside the mode it was made in)
+
+
+def test_an_error_of_an_earlier_call_is_left_where_it_is():
+    """The program's own failed HIP call, whose error it has not fetched yet, is not an operator's, and is still there afterwards"""
+    with open("/proc/self/maps") as f:
+        hip = ctypes.CDLL(next(line.split()[-1] for line in f if "libamdhip64" in line))
+    x = torch.randn(4, 64, device="cuda")
+    (codes, s), (wide, ws) = ops.quantize(x), ops.quantize(torch.randn(100, 64, device="cuda"))
+    pos, f = torch.zeros(4, device="cuda", dtype=torch.int32), torch.ones(16, device="cuda").double()
+    y, q, out, codes_out = torch.empty_like(x), torch.empty(4, 2, 32, device="cuda"), torch.empty(4, 4, device="cuda"), torch.empty(100, 4, device="cuda")
+    lib, stream = capi.load_library(), torch.cuda.current_stream().cuda_stream
+    calls = [lambda: ops.rms_norm(x, y_out=y), lambda: ops.linear8(codes, s, codes, s, out=out), lambda: ops.linear8(wide, ws, codes, s, out=codes_out),
+             lambda: ops.rotary(x.reshape(4, 2, 32), None, pos, f, q_out=q),
+             lambda: lib.kmx_quantize(0, ctypes.c_void_p(stream), capi.PREC_FP32, 1, 4, 64, x.data_ptr(), 64, codes.data_ptr(), 64, s.data_ptr()) and pytest.fail()]
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        try:
+            left = hip.hipSetDevice(9999)
+            assert left != 0
+            call()
+            still = hip.hipPeekAtLastError()
+        finally:
+            hip.hipGetLastError()
+        assert still == left
+    torch.cuda.synchronize()
