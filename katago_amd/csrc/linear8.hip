@@ -4,10 +4,12 @@
 // Two ways to multiply, by the output's type:
 //   16-bit outputs  v_mfma_scale_f32_32x32x64_f8f6f4 on the codes (2048 flop a cycle and SIMD; e8m0 scales are its operands). Its adder
 //                   brings 8 products at a time to the largest one's exponent and keeps 13 bits below it, then adds those sums in fp32 (measured
-//                   with a product of 2^16 beside one of 2^e: 2^3 still counts, 2^2 does not). Over a row that is 1.4e-5 of the result (7e-5 with
-//                   a few channels 400 times the others): 1/3 of an fp16 rounding at worst.
-//   fp32 outputs    the codes, times their e8m0 scale, are exact bf16 numbers (4 significant bits): v_mfma_f32_32x32x16_bf16, all sums in
-//                   fp32, at half the rate.
+//                   with a product of 2^16 beside one of 2^e: 2^3 still counts, 2^2 does not): a result is off by up to 7 * 2^-13 of the sum of its
+//                   products' magnitudes, relative to itself by more where they cancel. Over random rows it was 1.4e-5 of the results' norm
+//                   (7e-5 with a few channels 400 times the others), where an fp16 rounding is 2.8e-4.
+//   fp32 outputs    the codes, times their e8m0 scale, as bf16 numbers: v_mfma_f32_32x32x16_bf16, all sums in fp32, at half the rate. 4
+//                   significant bits are exact there with scales from 2^-124 (bf16 reaches down to 2^-133, the smallest code is 2^-9) to 2^119
+//                   (448 * 2^119 < 2^128). An e8m0 scale beyond these belongs to values that fp32 itself does not hold, or barely.
 //
 // Long k is bound by the matrix cores and the LDS that feeds them: 8192^3 with row scales 408 us (2690 TFLOP/s; a large library product in 8 bits
 // reaches 2330 with scales by row, 2810 with one for all), 8190 x 11008 x 4096 with scales for 32 k each 327 us (2260), the same into fp32 730 us (1010).

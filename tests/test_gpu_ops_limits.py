@@ -9,7 +9,7 @@ import ops_ref as ref
 from katago_amd import capi, ops
 from katago_amd.capi import KatamxError
 from test_gpu_ops import eight, gen
-from test_ops_limits_emulated import check_linear_any, check_small_results, rounded_quotients, rows_of_any_size, small_sine_angles, spread_scales
+from test_ops_limits_emulated import check_block_scales, check_linear_any, check_small_results, rounded_quotients, rows_of_any_size, small_sine_angles, spread_scales
 
 pytestmark = pytest.mark.gpu
 
@@ -175,3 +175,10 @@ def test_an_error_of_an_earlier_call_is_left_where_it_is():
             hip.hipGetLastError()
         assert still == left
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 512), (30, 100, 4096), (64, 64, 288), (70, 64, 512), (361, 1152, 384), (1000, 4100, 1152), (5000, 4999, 512)])
+def test_linear8_block_scales_at_their_ends(m, n, k):
+    def run(a, sa, w, sw, out):
+        return ops.linear8(a.cuda(), sa.cuda(), w.cuda(), sw.cuda(), out_dtype=ref.TYPES[out]).cpu()
+    check_block_scales(run, m, n, k, torch.Generator().manual_seed(m + k))

@@ -147,3 +147,29 @@ def test_rotary_of_small_sines(emu):  # noqa: F811
     out, pos, f = torch.empty_like(q), torch.ones(1, 1, 1, dtype=torch.int32), angle.reshape(n, 1, 1)
     ok(emu, emu.kmx_rotary(0, None, ctypes.byref(rotary_args(q, None, out, None, pos, f, "fp32", False, 1.0, False))))
     check_small_results(out.reshape(n, 2, 2), angle)
+
+
+def block_scales(m, n, k, low, high, gen):
+    """e8m0 codes of two matrices whose blocks of 32 are as far apart as `low` .. `high` allow and whose products are ordinary numbers"""
+    e = torch.randint(low, high + 1, (k // 32,), generator=gen)
+    e[:2] = torch.tensor([low, high])
+    sa, sw = e.expand(m, -1), (low + high - e).expand(n, -1)
+    near = torch.randint(0, 2, (n, k // 32), generator=gen)
+    sw = (sw + near).clamp(max=high)
+    return sa.to(torch.uint8).contiguous().view(torch.float8_e8m0fnu), sw.to(torch.uint8).contiguous().view(torch.float8_e8m0fnu)
+
+
+def check_block_scales(run, m, n, k, gen):
+    """run(a, sa, w, sw, out type) over the scales that each output's way takes: all of e8m0 but NaN into 16 bits, 2^-124 .. 2^119 into fp32"""
+    a, w = (torch.randint(0, 256, (r, k), generator=gen).to(torch.uint8) for r in (m, n))
+    for c in (a, w):
+        c[c & 0x7f == 0x7f] = 0x3a
+    a, w = a.view(torch.float8_e4m3fn), w.view(torch.float8_e4m3fn)
+    for out, low, high in (("fp32", 3, 246), ("bf16", 0, 254)):
+        sa, sw = block_scales(m, n, k, low, high, gen)
+        check_linear_any(run(a, sa, w, sw, out), *ref.linear(ref.values(a, sa), ref.values(w, sw)), k)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 512), (20, 33, 96), (70, 64, 512), (130, 70, 288)])
+def test_linear8_block_scales_at_their_ends(emu, m, n, k):  # noqa: F811
+    check_block_scales(lambda a, sa, w, sw, out: linear(emu, a, sa, w, sw, out, 2), m, n, k, torch.Generator().manual_seed(m + k))
