@@ -1,11 +1,14 @@
 """-m gpu: katago_amd.ops at the ends of what it takes - scales, values, lengths and tensors far from the usual ones - against plain formulas in 64 bits."""
 import ctypes
+import subprocess
+import sys
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import ops_ref as ref
+from conftest import REPO
 from katago_amd import capi, ops
 from katago_amd.capi import KatamxError
 from test_gpu_ops import eight, gen
@@ -182,3 +185,63 @@ def test_linear8_block_scales_at_their_ends(m, n, k):
     def run(a, sa, w, sw, out):
         return ops.linear8(a.cuda(), sa.cuda(), w.cuda(), sw.cuda(), out_dtype=ref.TYPES[out]).cpu()
     check_block_scales(run, m, n, k, torch.Generator().manual_seed(m + k))
+
+
+@pytest.mark.parametrize("out", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("scales", ["row", "mx"])
+@pytest.mark.parametrize("m,n,k", [(1000, 3900, 1152), (700, 3300, 1056), (5000, 4999, 1152), (4096, 4096, 1664), (4000, 4090, 1184), (1, 4096, 11008), (7, 70, 8224), (30, 100, 11008),
+                                   (64, 130, 11008), (300, 2000, 11008), (1200, 1300, 8224)])
+def test_linear8_of_long_k(m, n, k, scales, out):
+    """Tiles of 128 x 128 with four stages, tiles of 256 x 256 whose k has steps between its first and its last ones, k of several rounds of the kernel for
+    few rows"""
+    g = gen(m + n)
+    (a, sa), (w, sw) = eight(m, k, scales, g, 2.0), eight(n, k, scales, g, 0.1)
+    b = torch.randn(n, device="cuda", generator=g) if (m + n) % 2 else None
+    buf = torch.full((m, n + 9), 7.0, device="cuda", dtype=ref.TYPES[out])
+    y = ops.linear8(a, sa, w, sw, b, out=buf[:, 1:n + 1])
+    ref.check_linear(y, *ref.linear(ref.values(a, sa), ref.values(w, sw), b), k)
+    assert bool((buf[:, 0] == 7).all()) and bool((buf[:, n + 1:] == 7).all())
+
+
+def test_the_first_call_of_a_process_may_be_a_captured_large_tile():
+    """Tiles of 256 x 256 (8192 x 4096 x 256) and of 128 x 128 (1100 rows), whose launches opt in to their LDS, with nothing loaded before they are recorded"""
+    code = r"""
+import sys, torch
+sys.path.insert(0, %r)
+from katago_amd import ops
+with torch.no_grad():
+    x, m, t = torch.randn(8192, 256, device="cuda").half(), torch.randn(4096, 256, device="cuda").half(), torch.randn(1100, 256, device="cuda").half()
+    def run():
+        (a, sa), (w, sw) = ops.quantize(x, "mx"), ops.quantize(m, "mx")
+        return ops.linear8(a, sa, w, sw), ops.linear8(*ops.quantize(t, "mx"), w, sw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        x.normal_()
+        t.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        far = (got[0].double() - x.double() @ m.double().t()).norm() / got[0].double().norm()
+        assert float(far) < 0.051  # an e4m3 rounding in each factor
+print("FIRST_OK")
+""" % REPO
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "FIRST_OK" in r.stdout, r.stdout[-1000:] + r.stderr[-3000:]
+
+
+def test_rotary_of_more_threads_than_a_launch_counts():
+    """700 times the same million tokens, a thread for each of their three pairs: more than 2^31 threads, in two launches"""
+    g = gen(5)
+    S, B = 1 << 20, 700
+    x = torch.randn(1, S, 1, 6, device="cuda", generator=g).half()
+    pos, f = torch.randint(0, 1000, (S,), device="cuda", generator=g), torch.rand(3, device="cuda", generator=g, dtype=torch.float64)
+    out = torch.full((B + 1, S, 1, 6), 7.0, device="cuda", dtype=torch.float16)
+    ops.rotary(x.expand(B, S, 1, 6), None, pos, f, q_out=out[:B])
+    ref.check_rotary(out[0], *ref.rotary(x[0], pos[:, None], f[None, None], False))
+    for b in range(1, B):
+        assert torch.equal(out[b], out[0]), b
+    assert bool((out[B] == 7).all())
