@@ -96,7 +96,12 @@ hipError_t computeUnits(int device, int* n) { return hipDeviceGetAttribute(n, hi
 constexpr int CUS = 256;  // of the chip: what the choice of a kernel was measured on
 #ifdef KMX_EMULATED_HIP
 constexpr int PER_XCD = 2, SHORT_TILES = 2;  // (few rows are many)
+inline int chosenFor() {  // (few tiles are more than such a chip holds: the large ones are chosen, and go round)
+  const char* const e = getenv("KMX_EMU_CUS");
+  return e != nullptr ? atoi(e) : CUS;
+}
 #else
+constexpr int chosenFor() { return CUS; }
 constexpr int PER_XCD = CUS / 8 * 2, SHORT_TILES = 10;  // linear8ShortKernel: work-groups of an XCD, tiles of each at least
 #endif
 
@@ -496,9 +501,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     const float* const sc = scalesOf + parity * (BM + BN);
     bool ok = true;
 #pragma unroll
-    for(int r = lane; r < TM; r += 64) ok = mild(sc[wm * TM + r]) && ok;
+    for(int r = 0; r < TM; r += 64) ok = (r + lane >= TM || mild(sc[wm * TM + r + lane])) && ok;
 #pragma unroll
-    for(int c = lane; c < TN; c += 64) ok = mild(sc[BM + wn * TN + c]) && ok;
+    for(int c = 0; c < TN; c += 64) ok = (c + lane >= TN || mild(sc[BM + wn * TN + c + lane])) && ok;
     return !anyLane(!ok);
   };
 
@@ -1027,7 +1032,7 @@ hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
   // k = 384: n = 1152 in 84 us against 89, but n = 384, half of its second tile empty, in 34 against 28); the small one while there is a
   // round of it - with one work-group to a CU four stages, which hide a request's time better (1000 x 4096 x 4096 27.1 -> 24.0 us);
   // below that 64 x 64, with four stages where k is long (128 x 4096 x 4096 16.8 -> 10.0 us, 361 x 1152 x 384 3.8 -> 4.9).
-  const int64_t cus = CUS;
+  const int64_t cus = chosenFor();
   auto tiles = [&](int b) { return (g.rows + b - 1) / b * ((g.N + b - 1) / b); };
   const int64_t large = tiles(256), small = tiles(128);
   if constexpr(OUT != DT_F32)

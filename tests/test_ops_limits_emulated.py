@@ -1,11 +1,15 @@
 """The ends of what include/katamx_ops.h takes - scales, values and lengths far from the usual ones - through the kernels compiled for x86
 (tests/fakehip/emulate_ops.cpp), against plain formulas in 64 bits."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import ops_ref as ref
+from conftest import REPO
 from katago_amd import capi
 from test_ops_emulated import PREC, Guarded, aligned_copy, eight, emu, ok, rotary_args  # noqa: F401 (emu: the fixture)
 
@@ -173,3 +177,26 @@ def check_block_scales(run, m, n, k, gen):
 @pytest.mark.parametrize("m,n,k", [(3, 40, 512), (20, 33, 96), (70, 64, 512), (130, 70, 288)])
 def test_linear8_block_scales_at_their_ends(emu, m, n, k):  # noqa: F811
     check_block_scales(lambda a, sa, w, sw, out: linear(emu, a, sa, w, sw, out, 2), m, n, k, torch.Generator().manual_seed(m + k))
+
+
+@pytest.mark.parametrize("mode", ["0", "1", "2"])
+def test_linear8_large_tiles(emu, mode):  # noqa: F811
+    """Tiles of 256 x 256 and of 128 x 128 with two stages and with four, which a chip of 256 CUs takes for far larger products: whole ones and partial ones,
+    work-groups that go round several, k with steps between the first and the last ones. With copies into LDS that land at once (0), only when a wait requires
+    it (1), or at the barrier behind that wait (2)."""
+    code = r"""
+import ctypes, os, sys
+sys.path[:0] = [%r, %r]
+import test_ops_emulated as t
+lib = ctypes.CDLL(%r)
+t.capi.bind_ops(lib)
+lib.kmx_last_error.restype = ctypes.c_char_p
+for cus, case in [("1", (768, 1024, 896, "row", "fp16", True)), ("1", (760, 1000, 672, "mx", "bf16", False)), ("1", (400, 600, 1168, "row", "fp32", True)),
+                  ("1", (384, 384, 288, "mx", "fp32", False)), ("18", (384, 640, 1152, "row", "bf16", False)), ("18", (380, 600, 1184, "mx", "fp16", True))]:
+    os.environ["KMX_EMU_CUS"] = cus
+    print(cus, case, flush=True)
+    t.test_linear8(lib, *case)
+print("TILES_OK")
+""" % (REPO, os.path.join(REPO, "tests"), emu._name)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=dict(os.environ, KMX_EMU_LATE_DMA=mode))
+    assert r.returncode == 0 and "TILES_OK" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
