@@ -29,7 +29,7 @@ extern "C" {
 int kmx_ops_version(void);
 
 /* How a row of e4m3 codes is scaled; value = code * scale.
- *   ROW: float[rows], scale = max(amax / 448, 2^-126) of the row, 1 for a row of zeros
+ *   ROW: float[rows], scale = max(amax / 448, 2^-126) of the row, rounded to fp32 once the codes are made; 1 for a row of zeros
  *   MX:  uint8[rows][channels / 32], e8m0: 2^(code - 127) for 32 channels each, the smallest power of two (from 2^-127) that brings them
  *        to at most 448, 1 (code 127) where all are 0. channels is a multiple of 32.
  * A row (a block) that holds an infinity or a NaN has the scale NaN (code 255) and codes 0: it stays NaN in whatever it is multiplied with. */

@@ -79,17 +79,17 @@ def test_rms_norm_of_a_very_long_row(c):
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 def test_codes_are_rounded_quotients(dtype):
-    """16-bit values lie on the border of two codes often enough that a product with the rounded reciprocal is told from the quotient; what a norm
-    codes is its fp32 result"""
+    """16-bit values lie on the border of two codes often enough that a product with the rounded reciprocal, or a quotient by the rounded scale, is told from
+    the formula's quotient; what a norm codes is its fp32 result"""
     g, t = gen(3), ref.TYPES[dtype]
     for rows, c in ((16383, 1536), (361, 384), (5, 8190), (3, 70000)):
         x = (torch.randn(rows, c, device="cuda", generator=g) * 3).to(t)
         codes, s = ops.quantize(x)
         assert torch.equal(s, (x.abs().amax(1).double() / 448).float())  # (torch multiplies a device tensor with 1 / 448)
-        assert torch.equal(codes.view(torch.uint8), rounded_quotients(x, s))
+        assert torch.equal(codes.view(torch.uint8), rounded_quotients(x))
         if dtype == "fp32":
             n = ops.rms_norm(x, scales="row", want_y=True)
-            assert torch.equal(n.codes.view(torch.uint8), rounded_quotients(n.y, n.scales))
+            assert torch.equal(n.codes.view(torch.uint8), rounded_quotients(n.y))
 
 
 @pytest.mark.parametrize("layout", ["half", "interleaved"])

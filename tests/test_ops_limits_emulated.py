@@ -107,21 +107,23 @@ def test_rms_norm_of_a_very_long_row(emu):  # noqa: F811
     ref.check_y(y, ref.norm(x, eps=0.0)[1])
 
 
-def rounded_quotients(v, scales):
-    """e4m3(v / scale): the quotient rounded to fp32 (by way of 64 bits, which rounds no quotient of fp32 numbers otherwise), and that to nearest even"""
-    return (v.double() / scales.double()[:, None]).float().clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+def rounded_quotients(v):
+    """e4m3(v / (amax / 448)): the formula in 64 bits, its quotient rounded to fp32 (which restores one that lies on the border of two codes) and to e4m3"""
+    v = v.double()
+    return (v / (v.abs().amax(1, keepdim=True) / 448)).float().clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
-def test_quantize_divides(emu, dtype):  # noqa: F811
-    """16-bit values lie on the border of two codes often enough that a product with the rounded reciprocal is told from the quotient"""
+def test_quantize_divides_as_the_formula(emu, dtype):  # noqa: F811
+    """16-bit values lie on the border of two codes often enough that a product with the rounded reciprocal, or a quotient by the rounded scale, is told from
+    the formula's quotient"""
     g, t = torch.Generator().manual_seed(3), ref.TYPES[dtype]
     for rows, c in ((400, 512), (3, 40000)):
         x = torch.randn(rows, c, generator=g).to(t)
         codes, sc = torch.zeros(rows, c, dtype=torch.uint8), torch.zeros(rows)
         ok(emu, emu.kmx_quantize(0, None, PREC[dtype], 1, rows, c, x.data_ptr(), c, codes.data_ptr(), c, sc.data_ptr()))
         assert torch.equal(sc, x.float().abs().amax(1) / 448)
-        assert torch.equal(codes, rounded_quotients(x, sc))
+        assert torch.equal(codes, rounded_quotients(x))
 
 
 def small_sine_angles():
