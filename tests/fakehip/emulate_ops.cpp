@@ -6,6 +6,32 @@
 
 #include <stdexcept>
 
+// Three devices, of which a thread has a current one; a launch notes which that was
+namespace emu {
+inline thread_local int currentDevice = 0, launchedOn = -1;
+inline hipError_t countDevices(int* n) {
+  *n = 3;
+  return hipSuccess;
+}
+inline hipError_t getDevice(int* d) {
+  *d = currentDevice;
+  return hipSuccess;
+}
+inline hipError_t setDevice(int d) {
+  if(d < 0 || d >= 3) return hipErrorInvalidDevice;
+  currentDevice = d;
+  return hipSuccess;
+}
+}  // namespace emu
+#define hipGetDeviceCount emu::countDevices
+#define hipGetDevice emu::getDevice
+#define hipSetDevice emu::setDevice
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kern, grid, block, lds, stream, ...) (emu::launchedOn = emu::currentDevice, emu::launchImpl(grid, block, [&] { kern(__VA_ARGS__); }))
+extern "C" int emu_launched_on(void) { return emu::launchedOn; }
+extern "C" int emu_current_device(void) { return emu::currentDevice; }
+extern "C" void emu_make_current(int device) { emu::currentDevice = device; }
+
 namespace emu {
 inline float decodeE4m3(unsigned v) {
   const unsigned e = (v >> 3) & 15, m = v & 7;

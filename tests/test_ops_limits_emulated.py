@@ -202,3 +202,34 @@ print("TILES_OK")
 """ % (REPO, os.path.join(REPO, "tests"), emu._name)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=dict(os.environ, KMX_EMU_LATE_DMA=mode))
     assert r.returncode == 0 and "TILES_OK" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
+
+
+def test_calls_on_another_device_than_the_current_one(emu):  # noqa: F811
+    """A launch is made with the call's device current, and the thread's own is current again behind it, behind refusals too"""
+    g = torch.Generator().manual_seed(1)
+    x, codes, sc = torch.randn(70, 64, generator=g), torch.zeros(70, 64, dtype=torch.uint8), torch.zeros(70)
+    y, rot = torch.zeros(70, 64), torch.zeros(1, 70, 1, 64)
+    a, sa = eight(70, 64, "row", g)
+    buf, p = aligned_copy(a, 64)
+    out = torch.zeros(70, 70)
+    norm = capi.RmsNormArgs(type=capi.PREC_FP32, rows=70, channels=64, epsilon=1e-6, x=x.data_ptr(), y=y.data_ptr(), x_stride=64, y_stride=64)
+    lin = capi.Linear8Args(out_type=capi.PREC_FP32, scale_kind=1, rows=70, n=70, k=64, a=p, a_scales=sa.data_ptr(), w=p, w_scales=sa.data_ptr(), out=out.data_ptr(),
+                           a_stride=64, w_stride=64, out_stride=70)
+    pos, f = torch.zeros(1, 70, 1, dtype=torch.int32), torch.ones(1, 1, 32, dtype=torch.float64)
+    turn = rotary_args(x.reshape(1, 70, 1, 64), None, rot, None, pos, f, "fp32", False, 1.0, False)
+    calls = [lambda d: emu.kmx_rmsnorm(d, None, ctypes.byref(norm)), lambda d: emu.kmx_linear8(d, None, ctypes.byref(lin)), lambda d: emu.kmx_rotary(d, None, ctypes.byref(turn)),
+             lambda d: emu.kmx_quantize(d, None, capi.PREC_FP32, 1, 70, 64, x.data_ptr(), 64, codes.data_ptr(), 64, sc.data_ptr())]
+    try:
+        for current in (0, 2):
+            emu.emu_make_current(current)
+            for device in (1, 0, 2):
+                for call in calls:
+                    ok(emu, call(device))
+                    assert (emu.emu_launched_on(), emu.emu_current_device()) == (device, current)
+            for call in calls:
+                assert call(3) == capi.KMX_ERR_INVALID_ARG and emu.emu_current_device() == current
+    finally:
+        emu.emu_make_current(0)
+    ref.check_y(y, ref.norm(x)[1])
+    ref.check_linear(out, *ref.linear(ref.values(a, sa), ref.values(a, sa)), 64)
+    assert torch.equal(codes, rounded_quotients(x)) and torch.equal(rot.reshape(70, 64), x)
