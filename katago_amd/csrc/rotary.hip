@@ -206,7 +206,8 @@ hipError_t launchPieces(const RotaryArgs& a, hipStream_t stream) {
 template <class TR>
 hipError_t launchType(const RotaryArgs& a, hipStream_t stream) {
   // pieces of 16 bytes: 8 pairs of a 16-bit type, 4 of fp32 (8 of fp32 take 184 registers: 4 x 8191 x 9 heads of 64 in 34 us against 28)
-  if(sizeof(typename TR::T) == 2 && a.pairs % 8 == 0) return a.half ? launchPieces<TR, 8, true>(a, stream) : launchPieces<TR, 8, false>(a, stream);
+  if constexpr(sizeof(typename TR::T) == 2)
+    if(a.pairs % 8 == 0) return a.half ? launchPieces<TR, 8, true>(a, stream) : launchPieces<TR, 8, false>(a, stream);
   if(a.pairs % 4 == 0) return a.half ? launchPieces<TR, 4, true>(a, stream) : launchPieces<TR, 4, false>(a, stream);
   return a.half ? launchPieces<TR, 1, true>(a, stream) : launchPieces<TR, 1, false>(a, stream);
 }
