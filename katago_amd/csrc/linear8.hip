@@ -557,10 +557,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
     body(at++, step, STAGES - 2, step + 1, 0, Index<END>(), Index<0>());
     putScales(tileParity ^ 1);
     body(at++, step + 1, STAGES - 1, 0, 1, Index<END>(), Index<0>());
-    const bool plain = allMild(tileParity);
-    if(plain && tile.mLast == BM - 1 && tile.nLast == BN - 1) store(tile, tileParity, Index<1>(), Index<0>());
+    const bool plain = __builtin_expect(allMild(tileParity), 1);
+    if(__builtin_expect(plain && tile.mLast == BM - 1 && tile.nLast == BN - 1, 1)) store(tile, tileParity, Index<1>(), Index<0>());
     else {
-      if(plain) store(tile, tileParity, Index<0>(), Index<0>());
+      if(__builtin_expect(plain, 1)) store(tile, tileParity, Index<0>(), Index<0>());
       else store(tile, tileParity, Index<0>(), Index<1>());
       waitLoads<0>();  // (who knows how many of its lanes had something to store)
     }
