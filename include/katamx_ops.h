@@ -89,7 +89,8 @@ int kmx_linear8(int device, void* stream, const kmx_linear8_args* args);
  *   angle = sum over the axes of position[axis] * frequencies[head][axis][p]
  *   (u, v) -> magnitude * (u cos - v sin, u sin + v cos); `inverse` negates the angle (times magnitude^2 = 1 that undoes it; it is also
  *   the turn's transpose: what a gradient goes through)
- * in fp64 up to the angle's fraction of a turn, so positions of millions lose nothing. Channels from 2 pairs on are copied.
+ * in fp64 up to the angle's fraction of a turn, so positions of millions lose nothing; fp32 tensors turn with sines and cosines good to their last bits,
+ * 16-bit ones with such that are off by 2^-22 at most. Channels from 2 pairs on are copied.
  * q and k: [batch][seq][heads][head_dim] each, in and out; k_heads = 0: no k. out may be in itself (same pointer and strides), or a tensor that
  * overlaps nothing. positions: int32 or int64 [batch][seq][axes] by strides (0: the same for every sequence); frequencies: double
  * [freq_heads][axes][pairs], radians per position, contiguous, on the device. freq_heads is 1, or divides q_heads and k_heads: head h of H turns with

@@ -11,10 +11,10 @@
 //                   significant bits are exact there with scales from 2^-124 (bf16 reaches down to 2^-133, the smallest code is 2^-9) to 2^119
 //                   (448 * 2^119 < 2^128). An e8m0 scale beyond these belongs to values that fp32 itself does not hold, or barely.
 //
-// Long k is bound by the matrix cores and the LDS that feeds them: 8192^3 with row scales 408 us (2690 TFLOP/s; a large library product in 8 bits
-// reaches 2330 with scales by row, 2810 with one for all), 8190 x 11008 x 4096 with scales for 32 k each 327 us (2260), the same into fp32 730 us (1010).
-// Short k is bound by what surrounds the products, whose steps overlap in part: 92416 x 1152 x 384 68 us (3.7 TB/s; bytes alone: 49). Few rows are
-// bound by the weights' way in: 1 x 4096 x 4096 5.1 us (3.3 TB/s).
+// Long k is bound by the matrix cores and the LDS that feeds them: 8192^3 with row scales 380 to 395 us (2780 to 2890 TFLOP/s; a large library product in
+// 8 bits reaches 2330 with scales by row, 2810 with one for all), 8190 x 11008 x 4096 with scales for 32 k each 330 to 340 us (2170 to 2240), the same into fp32
+// 740 to 770 us (960 to 1000), 8191 x 11007 x 4096 with row scales 312 (2370). Short k is bound by what surrounds the products, whose steps overlap in
+// part: 92416 x 1152 x 384 62 us (4.0 TB/s; bytes alone: 49). Few rows are bound by the weights' way in: 1 x 4096 x 4096 5.0 us (3.4 TB/s), x 11008 10.1 (4.5).
 #include <atomic>
 
 #include "ops.h"
@@ -575,8 +575,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear8Kernel(Linear8Args g) 
 // Short k, many rows: a work-group keeps 128 output channels, whose weights stay in its waves' registers (64 channels of up to 384 k each), and goes down its
 // rows 128 at a time: only a's rows pass through LDS, in steps of 128 k, three of them on their way while one is multiplied. One barrier a step: behind
 // it the stage before has been read out by all and is requested anew. Two work-groups share a CU, so that one's products run beside the other's
-// results on their way out. The layouts are those of linear8Kernel; what lies beyond K has weights of zero. 92416 x 1152 x 384: 68 us (77 with linear8Kernel,
-// which fetches the weights anew for every tile), of which products alone take 39, the results' way through LDS 20; k = 128: 41 us, 5.4 TB/s.
+// results on their way out. The layouts are those of linear8Kernel; what lies beyond K has weights of zero. 92416 x 1152 x 384: 62 us (77 with linear8Kernel,
+// which fetches the weights anew for every tile), of which products alone take 39, the results' way through LDS 20; k = 128: 41 us, 5.4 TB/s. k of 384 takes 236
+// to 248 of the 256 registers that two work-groups to a CU leave a thread; 512 would need 64 more.
 template <int KS, bool MX, int OUT>
 __global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int groups) {
   typedef typename OutTraits<OUT>::TR TR;
@@ -840,7 +841,9 @@ __global__ __launch_bounds__(256, 2) void linear8ShortKernel(Linear8Args g, int 
   waitLoads<0>();  // (nothing may land in LDS that is another work-group's by then)
 }
 
-// Few rows: the time is the weights' way from memory, so they go straight into registers, every byte requested at once. A work-group owns 16 output
+// Few rows: the time is the weights' way from memory, so they go straight into registers, a wave's share of DEPTH steps in one round of requests. (With e8m0 scales
+// all of a round's requests are out before its first product; with row scales the compiler moves some behind it: 12 of 16 are out ahead for 16 rows, 6 of 12
+// for 32, 6 of 20 for 64. A second round is requested when the first has been multiplied.) A work-group owns 16 output
 // channels and up to 16 MT rows; its 8 waves take every eighth step of 128 k (v_mfma_scale_f32_16x16x128_f8f6f4, or four of 16x16x32_bf16) and add their
 // sums in LDS, in the order of the waves. Lane (r = l % 16, part = l / 16) holds k 16 part + [0, 16) and 64 + 16 part + [0, 16) of row r: 128
 // consecutive bytes of each weight row a step; the e8m0 code of block b comes from the lanes of part b.
@@ -1014,8 +1017,9 @@ hipError_t launchShape(const Linear8Args& g, hipStream_t stream) {
   // Few rows: up to 32 on the kernel without LDS (32 x 4096 x 4096 8.1 us; 64 rows 11.7 against 10.0 on 64 x 64 tiles with four stages), up to 64 where k
   // is too short for those to get going (64 x 1152 x 384 3.0 us against 3.8).
   const bool longK = g.K >= 8 * KSTEP;
-  // k that fits the registers, and rows enough: ten tiles of 128 rows to a work-group (12.9 of them, 92416 x 1152 x 384: 68 us against 77; 11.3, n = 1024:
-  // equal; 4.3, n = 384: 28 against 26.7; two, 14500 x 1152: 18.7 against 15.4)
+  // k that fits the registers, and rows enough: ten tiles of 128 rows to a work-group (12.9 of them, 92416 x 1152 x 384: 68 us against 77 when the rule was
+  // made; 11.3, n = 1024: equal; 4.3, n = 384: 28 against 26.7; two, 14500 x 1152: 18.7 against 15.4). About 512 work-groups share the chip, so that is 84
+  // million results and more.
   if constexpr(OUT != DT_F32) {
     const int64_t groups = PER_XCD / ((g.N + 127) / 128);  // of work-groups that share their rows, on an XCD
     if(g.K <= 3 * KSTEP && (!MX || g.K % KSTEP == 0) && groups >= 1 && (g.rows + 127) / 128 >= SHORT_TILES * 8 * groups) {

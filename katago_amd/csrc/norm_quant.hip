@@ -9,8 +9,9 @@
 // Everything between the loads and the stores is fp32; the sum of squares is fp64 where fp32's is not good enough. e4m3 rounds to nearest even.
 //
 // Bound by memory: a row's values stay in registers, so that everything is read once and written once. 92416 rows of 384 channels in fp16 with residual,
-// mask and codes 51 us (4.9 TB/s; a large copy reaches 5.1), 8190 of 4096 in bf16 with sum, y and codes for 32 channels each 56 us (5.4), the
-// 8-bit form alone of 16383 x 1536 15.6 us (4.9). A few rows are bound by one trip to memory and a launch: 361 x 384 3.3 us.
+// mask and codes 52 us (4.8 TB/s; a large copy reaches 5.1), 8190 of 4096 in bf16 with sum, y and codes for 32 channels each 55 us (5.5), the
+// 8-bit form alone of 16383 x 1536 17 us (4.4). A few rows are bound by one trip to memory and a launch: 361 x 384 4.2 us (3.6 in a graph).
+// With operands that the last call left in the caches: 92416 x 384 44 us, in fp32 84 (8190 x 4096 in fp32 78), 92416 x 383 57.
 #include "ops.h"
 #include "ops_device.h"
 
@@ -19,7 +20,7 @@ namespace kmx {
 namespace {
 
 // Vectors at element alignment: rows of any length start anywhere. gfx950 serves unaligned 16-byte accesses; aligned ones cost the same as with
-// an aligned type.
+// an aligned type (eight sizes, within 0.3 %), rows at odd addresses about a tenth more (92416 x 384 at a stride of 387 48.5 us against 44.3).
 typedef _Float16 h16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef __bf16 b16x8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef float f32x8u __attribute__((ext_vector_type(8), aligned(4)));
@@ -213,8 +214,8 @@ __device__ __forceinline__ Factor factorOf(double x) {
   const float t = xh * r, left = __builtin_fmaf(-t, r, 1.0f) - (__builtin_fmaf(xh, r, -t) + xl * r) * r, lo = 0.5f * r * left;
   return Factor{r, __builtin_fabsf(lo) < r * 1e-3f ? lo : 0.0f, pre};
 }
-// The norm's factor applied to 8 values: v * r * w, rounded once, + beta; 0 on a masked row. (Of 33.5 million codes 8 lie on the other side of a border than
-// the formula's in 64 bits; 15 with fp32's root and each product rounded. 256 boards take 1.3 us longer for it.)
+// The norm's factor applied to 8 values: v * r * w, rounded once, + beta; 0 on a masked row. (Of 35.5 million codes 8 lie on the other side of a border than
+// the formula's in 64 bits; 16 with fp32's root, each product and the scale rounded. 256 boards take 1.3 us longer for it.)
 __device__ __forceinline__ void scale8(const NormQuantArgs& a, int c, Factor r, bool on, float (&v)[8]) {
   if(!a.normed) return;
   float w[8];
@@ -418,7 +419,7 @@ hipError_t launchOne(const NormQuantArgs& a, hipStream_t stream) {
   const int pieces = (a.C + 7) / 8;
   // While the chip has a lane for every piece (1024 to a CU), each lane takes one: the call is one trip to memory and the row's exchanges, and
   // a lane's rounds would only add to it (361 rows of 384 channels 5.2 -> 3.3 us, of 2048 6.3 -> 3.8, one row of 8192 5.9 -> 3.9). More rows are
-  // faster on fewer lanes with several pieces each in flight (92416 rows of 384 42.7 us against 52).
+  // faster on fewer lanes with several pieces each in flight (92416 rows of 384 42.7 us against 52, operands in the caches).
   auto laneEach = [&](int lanes) { return a.rows * lanes <= 256 * 1024; };
   if(pieces <= 16) return launchRows<TR, 16, 1>(a, stream);
   if(pieces <= 64 && laneEach(64)) return launchRows<TR, 64, 1>(a, stream);

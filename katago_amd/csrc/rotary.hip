@@ -7,8 +7,9 @@
 // Angles are formed in fp64 and as turns (1 = 2 pi): a position of a million times a frequency near 1 has no correct bit left of its phase in
 // fp32; the turns' fraction is exact, and only then rounded. The rotation itself is fp32, rounded once.
 //
-// Bound by memory: 4 x 8191 tokens of 32 + 8 heads of 128 in bf16 124 us (5.4 TB/s; a large copy reaches 5.1), 256 boards of 12 + 6 heads of 32 in fp16
-// with learned frequencies 49 us (4.4). Eight tokens take 3.0 us, a launch and two trips to memory.
+// Bound by memory: 4 x 8191 tokens of 32 + 8 heads of 128 in bf16 123 us (5.4 TB/s; a large copy reaches 5.1), 256 boards of 12 + 6 heads of 32 in fp16
+// with learned frequencies 44 us (4.8). Eight tokens take 3.7 us (3.0 in a graph), a launch and two trips to memory. Pairs that are no multiple of 4
+// go one to a thread, in pieces of 2 bytes: the same long sequences with 46 pairs of 64 take 213 us.
 #include "ops.h"
 #include "ops_device.h"
 

@@ -60,8 +60,9 @@ def rms_norm(x, weight=None, eps=1e-6, *, beta=None, residual=None, mask=None, s
         y     = sum / sqrt(mean(sum^2) + eps) * weight + beta; 0 on rows whose mask ([...], float32) is 0
         codes, scales = y in e4m3: scales="row" float32 [...], "mx" float8_e8m0fnu [..., channels / 32]; None: neither
 
-    want_y: whether y itself is returned (by default only without scales). weight and beta: float32 [channels]. sum_out / y_out: the tensors to write,
-    each may be x or residual itself. Returns Normed(sum, y, codes, scales), None for what was not asked for."""
+    want_y: whether y itself is returned (by default only without scales). weight and beta: float32 [channels]. x's rows (and every other tensor's) lie at one
+    stride, whatever their leading dimensions are: x[:, 1:4] of a [2, 5, channels] tensor does not and is refused. sum_out / y_out: the tensors to write, each may be
+    x or residual itself. Returns Normed(sum, y, codes, scales), None for what was not asked for."""
     kind = SCALES.get(scales, -1)
     if kind < 0:
         _refuse("scales must be None, 'row' or 'mx'")
@@ -69,7 +70,7 @@ def rms_norm(x, weight=None, eps=1e-6, *, beta=None, residual=None, mask=None, s
 
 
 def quantize(x, scales="row"):
-    """(codes, scales) of x's rows ([..., channels]) in e4m3: what linear8 multiplies. scales as in rms_norm."""
+    """(codes, scales) of x's rows ([..., channels], at one stride) in e4m3: what linear8 multiplies. scales as in rms_norm."""
     if scales != "row" and scales != "mx":
         _refuse("scales must be 'row' or 'mx'")
     return (_native or _load()).quantize(x, SCALES[scales])
@@ -78,7 +79,8 @@ def quantize(x, scales="row"):
 def linear8(codes, scales, weight_codes, weight_scales, bias=None, *, out_dtype=torch.float16, out=None):
     """[..., n] = (codes * scales) (weight_codes * weight_scales)^T + bias: codes e4m3 [..., k], weight_codes e4m3 [n, k], scales of both as
     rms_norm / quantize return them (of one kind), bias float32 [n]. k is a multiple of 16 (mx: 32). out_dtype float16, bfloat16 or float32; float32
-    is summed in fp32 throughout, the others on the 8-bit matrix instructions (katamx_ops.h)."""
+    is summed in fp32 throughout (mx: scales from 2^-124 to 2^119), the others on the 8-bit matrix instructions (katamx_ops.h). out: the tensor to write, in its
+    own type."""
     return (_native or _load()).linear8(codes, scales, weight_codes, weight_scales, bias, out_dtype, out)
 
 
@@ -90,7 +92,8 @@ def rotary(q, k, positions, frequencies, *, layout="interleaved", magnitude=1.0,
     positions: int32 or int64, [batch, seq] / [tokens] (or [seq] for every sequence of a batch), and a last dimension of axes, which may be
     left out where there is one. frequencies: float64 [pairs], [axes, pairs] or [freq_heads, axes, pairs] on the device (rotary_frequencies(),
     board_frequencies()); freq_heads divides the heads of q and of k: query heads turn as the key head they read. inverse: the turn back, and
-    the transpose. q_out / k_out: the tensors to write, each may be q / k itself. Returns (q_out, k_out)."""
+    the transpose. float32 tensors turn with sines and cosines good to their last bits, 16-bit ones with such that are off by 2^-22 at most. q_out / k_out:
+    the tensors to write, each may be q / k itself. Returns (q_out, k_out)."""
     if layout not in ("interleaved", "half"):
         _refuse("layout must be 'interleaved' or 'half'")
     return (_native or _load()).rotary(q, k, positions, frequencies, layout == "half", magnitude, inverse, q_out, k_out)
