@@ -8,7 +8,8 @@
 
 namespace kmx {
 
-// A launch, and ITS error: what an earlier call of the program left for hipGetLastError() stays there, and is not reported as this one's
+// A launch, and ITS error: what an earlier call of the program left for hipGetLastError() stays there, and is not reported as this one's. An error of the
+// launch is returned, and not left for others to find.
 template <class... P, class... A>
 hipError_t launchKernel(void (*kern)(P...), dim3 grid, dim3 block, int lds, hipStream_t stream, const A&... args) {
   static_assert(sizeof...(P) == sizeof...(A), "arguments");
@@ -19,7 +20,9 @@ hipError_t launchKernel(void (*kern)(P...), dim3 grid, dim3 block, int lds, hipS
   std::tuple<P...> copies(args...);
   return std::apply([&](P&... p) {
     void* at[] = {(void*)&p...};
-    return hipLaunchKernel((const void*)kern, grid, block, at, (size_t)lds, stream);
+    const hipError_t e = hipLaunchKernel((const void*)kern, grid, block, at, (size_t)lds, stream);
+    if(e != hipSuccess) (void)hipGetLastError();
+    return e;
   }, copies);
 #endif
 }
