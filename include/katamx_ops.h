@@ -67,7 +67,8 @@ int kmx_quantize(int device, void* stream, int type, int scale_kind, int64_t row
 
 /* out[m][n] = sum over k of a[m][k] w[n][k], both e4m3 with scales of one kind (ROW or MX, as the two calls above leave them), + bias[n];
  * a [rows][k], w [n][k], bias float[n] or NULL, out [rows][n] of out_type. k is a multiple of 16 (MX: of 32), a and w and their strides are
- * 16-byte aligned; n, k and the strides are below 2^23. Results leave fp32 on their way only where they leave it themselves.
+ * 16-byte aligned; n, k and the strides are below 2^23. With ROW scales, whatever their size, results leave fp32 on their way only
+ * where they leave it themselves.
  * 16-bit outputs are summed on the 8-bit matrix instructions, whose sums of 8 products keep 13 bits below the largest of them: a result is off by up to
  * 7 * 2^-13 of the sum of its products' magnitudes. fp32 outputs are summed in fp32 throughout, MX values code * scale as bf16 numbers: exact for scales
  * from 2^-124 to 2^119 (codes 3 to 246); beyond these a value of 2^128 or more is infinite, one below 2^-133 is lost. */
